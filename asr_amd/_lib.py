@@ -49,6 +49,15 @@ class ProjectorGrads(Structure):
     _fields_ = [(n, c_void_p) for n in ("gamma", "w1", "b1", "w2", "b2")]
 
 
+class KVCache(Structure):
+    _fields_ = [(n, c_int) for n in ("num_layers", "num_pages", "kv_heads", "head_dim", "num_seqs", "max_pages", "seq_stride")] + [
+        (n, c_void_p) for n in ("kv", "exps", "table", "lens", "starts", "refs", "status", "scratch")]
+
+
+KV_PAGE = 64
+KV_STATUS = {1: "the pool ran out of pages", 2: "a sequence would pass max_len", 4: "a negative token count",
+             8: "a parent that is no beam"}  # ASRK_KV_* bits
+
 _SIGNATURES = {
     # name: (restype, argtypes)
     "asrk_version": (c_int, []),
@@ -86,6 +95,18 @@ _SIGNATURES = {
                                    c_void_p]),
     "asrk_attention_bf16": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "asrk_attention_log2_bf16": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "asrk_beam_select_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "asrk_beam_select": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int, c_int, c_int64] + [c_void_p] * 7 + [c_size_t, c_void_p]),
+    "asrk_reorder_rows": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p]),
+    "asrk_kv_scratch_bytes": (c_size_t, [c_int, c_int]),
+    "asrk_kv_extend": (c_int, [POINTER(KVCache), c_void_p, c_int, c_void_p]),
+    "asrk_kv_reorder": (c_int, [POINTER(KVCache), c_void_p, c_int, c_void_p]),
+    "asrk_kv_compact": (c_int, [POINTER(KVCache), c_void_p]),
+    "asrk_kv_write": (c_int, [POINTER(KVCache), c_int, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "asrk_kv_read": (c_int, [POINTER(KVCache), c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "asrk_kv_attention_workspace_bytes": (c_size_t, [POINTER(KVCache), c_int, c_int, c_int]),
+    "asrk_kv_attention": (c_int, [POINTER(KVCache), c_int, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_float, c_void_p,
+                                  c_void_p, c_size_t, c_void_p]),
     "asrk_profile_enable": (c_int, [c_int]),
     "asrk_profile_read": (c_int, [c_int, POINTER(ctypes.c_double), POINTER(ctypes.c_double), POINTER(c_int), c_int]),
 }

@@ -1,0 +1,608 @@
+// The paged 8-bit key/value cache: its pages, and how tokens get in and out.
+//
+// A page holds 64 tokens of one key/value head, keys [64][D] and values transposed [D][64] (what the attention's matrix
+// instructions read without a shuffle), in e4m3 with one power-of-two scale each: x = q 2^e.  A power of two makes the
+// scaling itself exact: the only rounding is the one to e4m3's 3 bits (half a step, 2^-4 relative), every value held is
+// also a bf16 value, and when a later token raises the page's exponent the older ones are re-rounded exactly, but for
+// those that become subnormal.  e is the smallest integer with max|x| <= 448 2^e, clamped to [-64, 119]: at 119 the
+// largest value is 1.75 2^127, still a finite bf16 (larger inputs saturate there); below -64 everything is zero.
+// NaN and infinities are stored as NaN and take no part in the scale.
+//
+// Pages belong to sequences through `table`, with a count of holders per page (`refs`, 0 = free).  All of it lives on
+// the device, so that a decoding step needs no host round trip and can be captured into a graph.
+#include "asrk_kvcache.h"
+
+namespace {
+
+constexpr int MANAGE_T = 1024;  // threads of the one-workgroup kernels
+
+__device__ __forceinline__ int block_scan_exclusive(int v, int* lds, int& total) {  // MANAGE_T threads
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    if (lane == 63) lds[wave] = x;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < MANAGE_T / 64; ++w) {
+        const int t = lds[w];
+        before += w < wave ? t : 0;
+        total += t;
+    }
+    __syncthreads();
+    return before + x - v;
+}
+
+// The page that token `len` of a sequence goes into, if the sequence has it already; -1: a fresh one.
+__device__ __forceinline__ int open_page(const asrk_kv_cache& c, int64_t slot, int len) {
+    if (len % ASRK_KV_PAGE == 0) return -1;
+    const int page = c.table[slot * c.max_pages + len / ASRK_KV_PAGE];
+    return page < c.num_pages ? page : -1;
+}
+
+__device__ __forceinline__ int load_agent(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Scratch of the page kernels, in the caller's zero-initialised buffer (every call leaves the first two zero again).
+struct Scratch {
+    int *writers, *lowest, *list, *tmp, *moves, *count;
+    __host__ __device__ Scratch(int32_t* p, int64_t pages, int64_t slots) {
+        writers = p;               // [pages] sequences that write into the page
+        lowest = writers + pages;  // [pages] (slots - index) of the first of them
+        list = lowest + pages;     // [pages] pages to hand out / new number of a page
+        tmp = list + pages;        // [slots][2]
+        moves = tmp + 2 * slots;   // [max(slots, pages)][2] page copies: source, target
+        count = moves + 2 * (slots > pages ? slots : pages);
+    }
+};
+
+// Lists up to `want` pages, in ascending order from `from` (below `to`), whose holders are none (FREE) or some; returns how many there are.
+template <bool FREE>
+__device__ int list_pages(const int* refs, int from, int to, int want, int* out, int* lds) {
+    constexpr int PER = 16;
+    int found = 0;
+    for (int base = from; base < to && found < want; base += MANAGE_T * PER) {
+        const int at = base + threadIdx.x * PER;
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (at + i < to) mine |= (FREE == (refs[at + i] == 0) ? 1u : 0u) << i;
+        int total;
+        int r = found + block_scan_exclusive(__popc(mine), lds, total);
+        while (mine) {
+            const int i = __builtin_ctz(mine);
+            mine &= mine - 1;
+            if (r < want) out[r] = at + i;
+            ++r;
+        }
+        found += total;
+    }
+    return found < want ? found : want;
+}
+
+// Room for n[s] more tokens of every sequence: the lowest free pages, in the order of the sequences, and a page of its
+// own for a sequence that writes into one it shares -- the first of its holders keeps it if they all write.  All or
+// nothing: without enough pages (or with a count that does not fit) nothing is added and `status` says so.  One
+// workgroup: the work is a few integers per sequence and the order has to be total; ~10 us, once per step for all layers.
+__global__ __launch_bounds__(MANAGE_T) void kv_extend_kernel(asrk_kv_cache c, const int* __restrict__ n_each, int n_all) {
+    __shared__ int lds[MANAGE_T / 64];
+    __shared__ int flags, n_moves;
+    Scratch sc(c.scratch, c.num_pages, (int64_t)c.num_seqs * c.seq_stride);
+    const int S = c.num_seqs, M = c.max_pages;
+    if (threadIdx.x == 0) { flags = 0; n_moves = 0; }
+    __syncthreads();
+    for (int s = threadIdx.x; s < S; s += MANAGE_T) {  // who writes into which open page
+        const int64_t slot = (int64_t)s * c.seq_stride;
+        const int len = c.lens[slot], n = n_each ? n_each[s] : n_all;
+        if (n < 0) atomicOr(&flags, ASRK_KV_BAD_COUNT);
+        else if (n > (int64_t)M * ASRK_KV_PAGE - len) atomicOr(&flags, ASRK_KV_TOO_LONG);
+        else if (n > 0) {
+            const int page = open_page(c, slot, len);
+            if (page >= 0) {
+                atomicAdd(&sc.writers[page], 1);
+                atomicMax(&sc.lowest[page], S - s);
+            }
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    const bool fits = flags == 0;
+    __syncthreads();
+    int need_all = 0;
+    for (int base = 0; base < S && fits; base += MANAGE_T) {
+        const int s = base + threadIdx.x;
+        int need = 0, copy = 0;
+        if (s < S) {
+            const int64_t slot = (int64_t)s * c.seq_stride;
+            const int len = c.lens[slot], n = n_each ? n_each[s] : n_all;
+            need = (len + n + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE - (len + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
+            const int page = n > 0 ? open_page(c, slot, len) : -1;
+            if (page >= 0) {
+                const int refs = c.refs[page];
+                copy = refs > 1 && !(load_agent(&sc.writers[page]) == refs && load_agent(&sc.lowest[page]) == S - s);
+            }
+            need += copy;
+        }
+        int total;
+        const int begin = need_all + block_scan_exclusive(need, lds, total);
+        if (s < S) {
+            sc.tmp[2 * s] = begin;
+            sc.tmp[2 * s + 1] = copy;
+        }
+        need_all += total;
+    }
+    int got = 0;
+    if (fits && need_all > 0) {
+        got = need_all <= c.num_pages ? list_pages<true>(c.refs, 0, c.num_pages, need_all, sc.list, lds) : 0;
+        if (got < need_all && threadIdx.x == 0) flags = ASRK_KV_OUT_OF_PAGES;
+        __threadfence();
+        __syncthreads();
+    }
+    const bool go = fits && got == need_all;
+    for (int s = threadIdx.x; s < S; s += MANAGE_T) {
+        const int64_t slot = (int64_t)s * c.seq_stride;
+        const int len = c.lens[slot], n = n_each ? n_each[s] : n_all;
+        int* row = c.table + slot * M;
+        const int page = n > 0 && n <= (int64_t)M * ASRK_KV_PAGE - len ? open_page(c, slot, len) : -1;
+        if (page >= 0) {
+            sc.writers[page] = 0;
+            sc.lowest[page] = 0;
+            if (go && sc.tmp[2 * s + 1]) {
+                const int own = load_agent(&sc.list[sc.tmp[2 * s]]);
+                row[len / ASRK_KV_PAGE] = own;
+                c.refs[own] = 1;
+                atomicSub(&c.refs[page], 1);
+                const int m = atomicAdd(&n_moves, 1);
+                sc.moves[2 * m] = page;
+                sc.moves[2 * m + 1] = own;
+            }
+        }
+        if (go) {
+            int at = sc.tmp[2 * s] + sc.tmp[2 * s + 1];
+            for (int j = (len + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE; j < (len + n + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE; ++j, ++at) {
+                const int own = load_agent(&sc.list[at]);
+                row[j] = own;
+                c.refs[own] = 1;
+            }
+            c.lens[slot] = len + n;
+        }
+        c.starts[slot] = len;  // also if nothing was added: then no row is new
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sc.count[0] = n_moves;
+        if (flags) c.status[0] |= flags;
+    }
+}
+
+// The pages of a list (source, target), every layer: bytes and scales.
+__global__ __launch_bounds__(256) void kv_copy_pages_kernel(asrk_kv_cache c) {
+    const Scratch sc(c.scratch, c.num_pages, (int64_t)c.num_seqs * c.seq_stride);
+    const int n = sc.count[0];
+    const int64_t vecs = (int64_t)c.kv_heads * 2 * ASRK_KV_PAGE * c.head_dim / 16;  // 16-byte pieces of a page of one layer
+    const int64_t layer = (int64_t)blockIdx.y * c.num_pages;
+    for (int m = blockIdx.x; m < n; m += gridDim.x) {
+        const int64_t src = layer + sc.moves[2 * m], dst = layer + sc.moves[2 * m + 1];
+        const u32x4* a = (const u32x4*)c.kv + src * vecs;
+        u32x4* b = (u32x4*)c.kv + dst * vecs;
+        for (int64_t i = threadIdx.x + (int64_t)blockIdx.z * 256; i < vecs; i += 256 * gridDim.z) b[i] = a[i];
+        if (blockIdx.z == 0)
+            for (int h = threadIdx.x; h < c.kv_heads; h += 256) ((int*)c.exps)[dst * c.kv_heads + h] = ((const int*)c.exps)[src * c.kv_heads + h];
+    }
+}
+
+// Beam k of group b goes on from beam parents[b][k] of the same group (-1: from nothing, its pages are given back).
+// A thread owns one column of the group's table rows and reads all of it before it writes: in place, in one launch.
+constexpr int REORDER_MAX = 32;
+__global__ __launch_bounds__(64) void kv_reorder_kernel(asrk_kv_cache c, const int64_t* __restrict__ parents, int K) {
+    const int b = blockIdx.y;
+    const int M = c.max_pages;
+    const int j = blockIdx.x * 64 + threadIdx.x;
+    const int64_t* par = parents + (int64_t)b * K;
+    const int64_t first = (int64_t)b * K * c.seq_stride;
+    if (j < M) {
+        int now[REORDER_MAX], then[REORDER_MAX];
+#pragma unroll
+        for (int k = 0; k < REORDER_MAX; ++k)
+            if (k < K) {
+                const int64_t p = par[k];
+                now[k] = c.table[(first + (int64_t)k * c.seq_stride) * M + j];
+                then[k] = p == -1 ? -1 : (p < 0 || p >= K ? now[k] : c.table[(first + p * c.seq_stride) * M + j]);
+            }
+#pragma unroll
+        for (int k = 0; k < REORDER_MAX; ++k)
+            if (k < K && now[k] != then[k]) {
+                c.table[(first + (int64_t)k * c.seq_stride) * M + j] = then[k];
+                if (then[k] >= 0) atomicAdd(&c.refs[then[k]], 1);
+                if (now[k] >= 0) atomicSub(&c.refs[now[k]], 1);
+            }
+    }
+    if (blockIdx.x == 0) {  // one wave: all lengths are read before any is written
+        const int k = threadIdx.x;
+        int len = 0, start = 0;
+        if (k < K) {
+            int64_t p = par[k];
+            if (p < -1 || p >= K) {
+                atomicOr(&c.status[0], ASRK_KV_BAD_PARENT);
+                p = k;
+            }
+            if (p >= 0) {
+                len = c.lens[first + p * c.seq_stride];
+                start = c.starts[first + p * c.seq_stride];
+            }
+        }
+        __syncthreads();
+        if (k < K) {
+            c.lens[first + (int64_t)k * c.seq_stride] = len;
+            c.starts[first + (int64_t)k * c.seq_stride] = start;
+        }
+    }
+}
+
+// Compaction: the r-th page in use at or above the number of pages in use goes to the r-th free one below it, so
+// sources and targets are disjoint and all copies run at once.
+__global__ __launch_bounds__(MANAGE_T) void kv_compact_plan_kernel(asrk_kv_cache c) {
+    __shared__ int lds[MANAGE_T / 64];
+    Scratch sc(c.scratch, c.num_pages, (int64_t)c.num_seqs * c.seq_stride);
+    const int P = c.num_pages;
+    int mine = 0, used;
+    for (int p = threadIdx.x; p < P; p += MANAGE_T) {
+        mine += c.refs[p] > 0;
+        sc.list[p] = p;
+    }
+    block_scan_exclusive(mine, lds, used);
+    int* holes = sc.writers;  // both are zero between calls; they are cleared again below
+    int* high = sc.lowest;
+    const int n = list_pages<true>(c.refs, 0, used, used, holes, lds);
+    list_pages<false>(c.refs, used, P, n, high, lds);
+    __threadfence();
+    __syncthreads();
+    for (int r = threadIdx.x; r < n; r += MANAGE_T) {
+        const int src = load_agent(&high[r]), dst = load_agent(&holes[r]);
+        sc.moves[2 * r] = src;
+        sc.moves[2 * r + 1] = dst;
+        sc.list[src] = dst;
+        c.refs[dst] = c.refs[src];
+        c.refs[src] = 0;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < n; r += MANAGE_T) {
+        holes[r] = 0;
+        high[r] = 0;
+    }
+    if (threadIdx.x == 0) {
+        sc.count[0] = n;
+        c.status[1] = used;
+    }
+}
+__global__ __launch_bounds__(256) void kv_rename_kernel(asrk_kv_cache c) {
+    const Scratch sc(c.scratch, c.num_pages, (int64_t)c.num_seqs * c.seq_stride);
+    const int64_t n = (int64_t)c.num_seqs * c.seq_stride * c.max_pages;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int p = c.table[i];
+        if (p >= 0) {
+            const int q = sc.list[p];
+            if (q != p) c.table[i] = q;
+        }
+    }
+}
+
+// ---- tokens in
+
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float* x);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float* x) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
+}
+template <>
+__device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, float* x) {
+    const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+}
+
+__device__ __forceinline__ int exponent_of(float most) {  // smallest e with most <= 448 2^e, clamped
+    const uint32_t b = __float_as_uint(most);
+    const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return b == 0 ? ASRK_KV_EXP_MIN : (e < ASRK_KV_EXP_MIN ? ASRK_KV_EXP_MIN : (e > ASRK_KV_EXP_MAX ? ASRK_KV_EXP_MAX : e));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // normal range only
+
+// four values / scale -> four e4m3 bytes, to the nearest, ties to even; not finite: NaN
+__device__ __forceinline__ uint32_t to_e4m3x4(const float* x, float inv) {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i] * inv, -448.f, 448.f);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+    uint32_t u = (uint32_t)w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (!(fabsf(x[i]) < __builtin_inff())) u |= 0x7fu << (8 * i);
+    return u;
+}
+// four e4m3 bytes times 2^shift (shift <= 0), rounded again
+__device__ __forceinline__ uint32_t shift_e4m3x4(uint32_t u, float factor) {
+    float x[4];
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false);
+    const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, true);
+    x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
+    return to_e4m3x4(x, factor);
+}
+
+// One workgroup per (page that new tokens touch, head, sequence).  Two passes over the new rows (the second from cache):
+// the largest magnitude, then the bytes.  Older tokens of the page are only touched if the exponent grows.
+template <class T>
+__global__ __launch_bounds__(256) void kv_write_kernel(asrk_kv_cache c, const T* __restrict__ k, const T* __restrict__ v, int64_t seq_ld, int64_t row_ld,
+                                int64_t head_ld, int n, int64_t layer) {
+    __shared__ uint32_t most[2];
+    __shared__ int odd;
+    const int D = c.head_dim, H = c.kv_heads, M = c.max_pages;
+    const int s = blockIdx.z, h = blockIdx.y;
+    const int64_t slot = (int64_t)s * c.seq_stride;
+    const int start = c.starts[slot];
+    int rows = c.lens[slot] - start;
+    rows = rows < n ? rows : n;
+    const int pj = start / ASRK_KV_PAGE + blockIdx.x;
+    const int lo = start > pj * ASRK_KV_PAGE ? start : pj * ASRK_KV_PAGE;
+    const int hi = start + rows < (pj + 1) * ASRK_KV_PAGE ? start + rows : (pj + 1) * ASRK_KV_PAGE;
+    if (lo >= hi || pj >= M) return;
+    const int page = c.table[slot * M + pj];
+    if (page < 0 || page >= c.num_pages) return;
+    const int t0 = lo - pj * ASRK_KV_PAGE, t1 = hi - pj * ASRK_KV_PAGE;  // new tokens of this page: [t0, t1)
+    const int64_t at = ((layer * c.num_pages + page) * H + h);
+    uint8_t* kp = (uint8_t*)c.kv + at * 2 * ASRK_KV_PAGE * D;
+    uint8_t* vp = kp + ASRK_KV_PAGE * D;
+    int8_t* ep = c.exps + at * 4;
+    const int64_t base = (int64_t)s * seq_ld + (int64_t)h * head_ld - (int64_t)(start - pj * ASRK_KV_PAGE) * row_ld;  // row of token t: base + t * row_ld
+    const int old = *reinterpret_cast<const int*>(ep);
+    if (threadIdx.x < 2) most[threadIdx.x] = 0;
+    if (threadIdx.x == 0) odd = 0;
+    __syncthreads();
+    const int per = D / 8, units = (t1 - t0) * per;
+    float mk = 0.f, mv = 0.f;
+    bool nan_v = false;
+    for (int u = threadIdx.x; u < units; u += blockDim.x) {
+        const int64_t o = base + (int64_t)(t0 + u / per) * row_ld + (u % per) * 8;
+        float x[8], y[8];
+        load8(k + o, x);
+        load8(v + o, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float a = fabsf(x[i]), b = fabsf(y[i]);
+            mk = a < __builtin_inff() ? fmaxf(mk, a) : mk;
+            mv = b < __builtin_inff() ? fmaxf(mv, b) : mv;
+            nan_v |= !(b < __builtin_inff());
+        }
+    }
+    mk = wave_max(mk);
+    mv = wave_max(mv);
+    nan_v = __any(nan_v);
+    if ((threadIdx.x & 63) == 0) {
+        atomicMax(&most[0], __float_as_uint(mk));
+        atomicMax(&most[1], __float_as_uint(mv));
+        if (nan_v) atomicOr(&odd, 1);
+    }
+    __syncthreads();
+    int ek = exponent_of(__uint_as_float(most[0])), ev = exponent_of(__uint_as_float(most[1]));
+    const int ok = (int8_t)old, ov = (int8_t)(old >> 8);
+    float fk = 1.f, fv = 1.f;  // factor of the older tokens
+    if (t0 > 0) {
+        ek = ek > ok ? ek : ok;
+        ev = ev > ov ? ev : ov;
+        fk = pow2(ok - ek > -60 ? ok - ek : -60);  // 448 2^-60 is zero in e4m3 as well
+        fv = pow2(ov - ev > -60 ? ov - ev : -60);
+    }
+    const float ik = pow2(-ek), iv = pow2(-ev);
+    if (t0 > 0 && fk != 1.f)
+        for (int u = threadIdx.x; u < t0 * D / 4; u += blockDim.x) ((uint32_t*)kp)[u] = shift_e4m3x4(((const uint32_t*)kp)[u], fk);
+    for (int u = threadIdx.x; u < units; u += blockDim.x) {
+        const int t = t0 + u / per, d = (u % per) * 8;
+        float x[8];
+        load8(k + base + (int64_t)t * row_ld + d, x);
+        u32x2 w;
+        w[0] = to_e4m3x4(x, ik);
+        w[1] = to_e4m3x4(x + 4, ik);
+        *reinterpret_cast<u32x2*>(kp + t * D + d) = w;
+    }
+    // values: four tokens of one d at a time; lanes run over d, so that the rows are read in whole lines
+    const bool shift = t0 > 0 && fv != 1.f;
+    const int g0 = shift ? 0 : t0 / 4, g1 = (t1 + 3) / 4;
+    for (int u = threadIdx.x; u < (g1 - g0) * D; u += blockDim.x) {
+        const int d = u % D, g = g0 + u / D;
+        uint32_t* p = (uint32_t*)(vp + d * ASRK_KV_PAGE + g * 4);
+        float x[4];
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = g * 4 + i;
+            const bool in = t >= t0 && t < t1;
+            x[i] = in ? (float)v[base + (int64_t)t * row_ld + d] : 0.f;
+            mask |= in ? 0xffu << (8 * i) : 0;
+        }
+        uint32_t w = to_e4m3x4(x, iv);
+        if (mask != 0xffffffffu) {
+            uint32_t o = *p;
+            if (shift) o = shift_e4m3x4(o, fv);
+            w = (w & mask) | (o & ~mask);
+        }
+        *p = w;
+    }
+    if (threadIdx.x == 0) {
+        const int flag = odd | (t0 > 0 ? (old >> 16) & 1 : 0);
+        *reinterpret_cast<int*>(ep) = (ek & 0xff) | ((ev & 0xff) << 8) | (flag << 16);
+    }
+}
+
+// ---- tokens out
+
+// One workgroup per (page, head, layer and sequence) of the tokens [first, first + count) of every sequence.  The value
+// page is turned through LDS (rows of 68 bytes: 8 x 8 lanes read different banks).
+__global__ __launch_bounds__(256) void kv_read_kernel(asrk_kv_cache c, const int* __restrict__ first_each, int first_all, int count,
+                                                      int layer0, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out) {
+    __shared__ uint32_t turn[128 * 17];
+    const int D = c.head_dim, H = c.kv_heads, M = c.max_pages;
+    const int h = blockIdx.y;
+    const int s = blockIdx.z % c.num_seqs, l = blockIdx.z / c.num_seqs;
+    const int64_t slot = (int64_t)s * c.seq_stride;
+    const int64_t first = first_each ? first_each[s] : first_all;
+    const int64_t pj = (first < 0 ? -((-first + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE) : first / ASRK_KV_PAGE) + blockIdx.x;
+    const int64_t t_lo = first - pj * ASRK_KV_PAGE, t_hi = first + count - pj * ASRK_KV_PAGE;  // asked tokens within the page
+    if (t_hi <= 0) return;
+    const int lo = t_lo > 0 ? (int)t_lo : 0, hi = t_hi < ASRK_KV_PAGE ? (int)t_hi : ASRK_KV_PAGE;
+    if (lo >= hi) return;
+    int have = 0, page = -1;  // tokens that the page has
+    if (pj >= 0 && pj < M) {
+        const int64_t left = c.lens[slot] - pj * ASRK_KV_PAGE;
+        page = c.table[slot * M + pj];
+        have = page >= 0 && page < c.num_pages && left > 0 ? (left < ASRK_KV_PAGE ? (int)left : ASRK_KV_PAGE) : 0;
+    }
+    const int64_t at = (((int64_t)(layer0 + l) * c.num_pages + (have ? page : 0)) * H + h);
+    const uint8_t* kp = (const uint8_t*)c.kv + at * 2 * ASRK_KV_PAGE * D;
+    const uint8_t* vp = kp + ASRK_KV_PAGE * D;
+    const int e = *reinterpret_cast<const int*>(c.exps + at * 4);
+    const float sk = pow2((int8_t)e), sv = pow2((int8_t)(e >> 8));
+    const int64_t out0 = (((int64_t)l * c.num_seqs + s) * count - t_lo) * H * D + (int64_t)h * D;  // of token 0 of the page
+    const int per = D / 8;
+    if (have)
+        for (int u = threadIdx.x; u < D * 16; u += 256) turn[(u / 16) * 17 + u % 16] = ((const uint32_t*)vp)[u];
+    __syncthreads();
+    for (int u = threadIdx.x; u < (hi - lo) * per; u += 256) {
+        const int t = lo + u / per, d = (u % per) * 8;
+        bf16x8 y;
+        if (t < have) {
+            const u32x2 w = *reinterpret_cast<const u32x2*>(kp + t * D + d);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], sk, false);
+                const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], sk, true);
+                y[4 * i] = a[0]; y[4 * i + 1] = a[1]; y[4 * i + 2] = b[0]; y[4 * i + 3] = b[1];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = (bf16_t)0.f;
+        }
+        *reinterpret_cast<bf16x8*>(k_out + out0 + (int64_t)t * H * D + d) = y;
+    }
+    for (int u = threadIdx.x; u < 16 * per; u += 256) {  // four tokens, eight d
+        const int g = u / per, d = (u % per) * 8;
+        if (g * 4 >= hi || g * 4 + 4 <= lo) continue;
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = have ? turn[(d + i) * 17 + g] : 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int t = g * 4 + j;
+            if (t < lo || t >= hi) continue;
+            bf16x8 y;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = (bf16_t)0.f;
+            if (t < have) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const uint32_t two = ((w[i] >> (8 * j)) & 0xffu) | (((w[i + 1] >> (8 * j)) & 0xffu) << 8);
+                    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, sv, false);
+                    y[i] = a[0];
+                    y[i + 1] = a[1];
+                }
+            }
+            *reinterpret_cast<bf16x8*>(v_out + out0 + (int64_t)t * H * D + d) = y;
+        }
+    }
+}
+
+}  // namespace
+
+int asrk_kv_check(const asrk_kv_cache* c) {
+    if (!c || !c->kv || !c->exps || !c->table || !c->lens || !c->starts || !c->refs || !c->status || !c->scratch) return ASRK_ERR_NULL;
+    if (c->num_layers <= 0 || c->num_pages <= 0 || c->kv_heads <= 0 || c->num_seqs <= 0 || c->max_pages <= 0 || c->seq_stride <= 0)
+        return ASRK_ERR_SHAPE;
+    if (c->head_dim != 64 && c->head_dim != 128) return ASRK_ERR_SHAPE;
+    if (c->num_layers > 65535 || c->kv_heads > 65535 || c->num_seqs > 65535 || (int64_t)c->num_seqs * c->seq_stride > 0x7fffffff ||
+        c->max_pages > 0x7fffffff / ASRK_KV_PAGE || c->num_pages > 0x3fffffff)
+        return ASRK_ERR_SHAPE;
+    if (((uintptr_t)c->kv & 15) || ((uintptr_t)c->exps & 15) || ((uintptr_t)c->table & 3) || ((uintptr_t)c->lens & 3) ||
+        ((uintptr_t)c->starts & 3) || ((uintptr_t)c->refs & 15) || ((uintptr_t)c->status & 3) || ((uintptr_t)c->scratch & 15))
+        return ASRK_ERR_ALIGN;
+    return ASRK_OK;
+}
+
+extern "C" size_t asrk_kv_scratch_bytes(int num_pages, int num_slots) {
+    if (num_pages <= 0 || num_slots <= 0) return 0;
+    Scratch sc((int32_t*)nullptr, num_pages, num_slots);
+    return (size_t)(sc.count + 4 - (int*)nullptr) * sizeof(int32_t);
+}
+
+static void launch_copies(const asrk_kv_cache* c, int most, hipStream_t st) {
+    const int64_t bytes = (int64_t)c->kv_heads * 2 * ASRK_KV_PAGE * c->head_dim;
+    const int parts = (int)((bytes + 16383) / 16384);  // 16 KiB per workgroup and page
+    hipLaunchKernelGGL(kv_copy_pages_kernel, dim3(most < 512 ? most : 512, c->num_layers, parts < 64 ? parts : 64), dim3(256), 0, st, *c);
+}
+
+extern "C" int asrk_kv_extend(const asrk_kv_cache* c, const int32_t* n_each, int n_all, void* stream) {
+    if (int rc = asrk_kv_check(c)) return rc;
+    if (!n_each && n_all < 0) return ASRK_ERR_SHAPE;
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(kv_extend_kernel, dim3(1), dim3(MANAGE_T), 0, st, *c, n_each, n_all);
+    launch_copies(c, c->num_seqs, st);
+    return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
+}
+
+extern "C" int asrk_kv_reorder(const asrk_kv_cache* c, const int64_t* parents, int K, void* stream) {
+    if (int rc = asrk_kv_check(c)) return rc;
+    if (!parents) return ASRK_ERR_NULL;
+    if (K <= 0 || K > REORDER_MAX || c->num_seqs % K) return ASRK_ERR_SHAPE;
+    hipLaunchKernelGGL(kv_reorder_kernel, dim3((c->max_pages + 63) / 64, c->num_seqs / K), dim3(64), 0, (hipStream_t)stream, *c, parents, K);
+    return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
+}
+
+extern "C" int asrk_kv_compact(const asrk_kv_cache* c, void* stream) {
+    if (int rc = asrk_kv_check(c)) return rc;
+    if (c->seq_stride != 1) return ASRK_ERR_SHAPE;  // every table row has to be renamed
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(kv_compact_plan_kernel, dim3(1), dim3(MANAGE_T), 0, st, *c);
+    launch_copies(c, c->num_pages, st);
+    const int64_t blocks = ((int64_t)c->num_seqs * c->max_pages + 255) / 256;
+    hipLaunchKernelGGL(kv_rename_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, *c);
+    return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
+}
+
+extern "C" int asrk_kv_write(const asrk_kv_cache* c, int layer, const void* k, const void* v, int dtype, int64_t seq_ld, int64_t row_ld,
+                             int64_t head_ld, int n, void* stream) {
+    if (int rc = asrk_kv_check(c)) return rc;
+    if (!k || !v) return ASRK_ERR_NULL;
+    if (dtype != ASRK_F32 && dtype != ASRK_BF16) return ASRK_ERR_UNSUPPORTED;
+    if (layer < 0 || layer >= c->num_layers || n <= 0 || seq_ld < 0 || row_ld < 0 || head_ld < 0) return ASRK_ERR_SHAPE;
+    const int per = dtype == ASRK_F32 ? 4 : 8;  // values in 16 bytes
+    if (((uintptr_t)k & 15) || ((uintptr_t)v & 15) || seq_ld % per || row_ld % per || head_ld % per) return ASRK_ERR_ALIGN;
+    const dim3 grid((unsigned)(((int64_t)n + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1), c->kv_heads, c->num_seqs);
+    const dim3 block(n == 1 ? 64 : 256);  // a single token has D / 8 pieces of work per tensor
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == ASRK_F32)
+        hipLaunchKernelGGL(kv_write_kernel<float>, grid, block, 0, st, *c, (const float*)k, (const float*)v, seq_ld, row_ld, head_ld, n,
+                           (int64_t)layer);
+    else
+        hipLaunchKernelGGL(kv_write_kernel<bf16_t>, grid, block, 0, st, *c, (const bf16_t*)k, (const bf16_t*)v, seq_ld, row_ld, head_ld,
+                           n, (int64_t)layer);
+    return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
+}
+
+extern "C" int asrk_kv_read(const asrk_kv_cache* c, int layer, int layers, const int32_t* first_each, int first_all, int count, void* k_out,
+                            void* v_out, void* stream) {
+    if (int rc = asrk_kv_check(c)) return rc;
+    if (!k_out || !v_out) return ASRK_ERR_NULL;
+    if (layer < 0 || layers <= 0 || layer + (int64_t)layers > c->num_layers || count <= 0) return ASRK_ERR_SHAPE;
+    if (((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15)) return ASRK_ERR_ALIGN;
+    if ((int64_t)layers * c->num_seqs > 65535) return ASRK_ERR_SHAPE;
+    const dim3 grid((unsigned)(((int64_t)count + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1), c->kv_heads, c->num_seqs * layers);
+    hipLaunchKernelGGL(kv_read_kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, first_each, first_all, count, layer, (bf16_t*)k_out,
+                       (bf16_t*)v_out);
+    return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
+}

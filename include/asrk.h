@@ -242,6 +242,77 @@ int asrk_attention_bf16(const void* qkv, void* out, int B, int T, int H, void* s
 int asrk_attention_log2_bf16(const void* qkv, void* out, int B, int T, int H, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Decoding with beams.  The reference decodes through HF generate (src/modeling.py:329-334); these are the operators
+ * of that loop around the decoder's own layers: selection, the key/value cache, the attention over it.
+ * ---------------------------------------------------------------------------------------- */
+
+/* The best 2 K of the K V continuations of each utterance, c = scores[b][k] + log_softmax(logits[b K + k])[v], best
+ * first and ties to the lowest k V + v, as cand_* [B][2 K]; and the first K of them whose token is not `eos` (< 0: none),
+ * as out_* [B][K].  logits dev [B K] rows of V values (ASRK_F32 | ASRK_BF16) at a stride of ld values; scores dev f32
+ * [B][K].  Beams whose score or largest logit is not finite, or with a NaN logit, offer -inf.  K <= 16, 2 <= V,
+ * K V < 2^31, K ceil(V / 8192) <= 2048.  ws: dev scratch, 16-byte aligned. */
+size_t asrk_beam_select_workspace_bytes(int B, int K, int V);
+int asrk_beam_select(const void* logits, int dtype, int64_t ld, const float* scores, int B, int K, int V, int64_t eos,
+                     float* out_scores, int64_t* out_tokens, int64_t* out_parents, float* cand_scores, int64_t* cand_tokens,
+                     int64_t* cand_parents, void* ws, size_t ws_bytes, void* stream);
+
+/* out[b][k] = in[b][parents[b][k]] for rows of row_bytes bytes (a parent that is no beam: the row itself); parents dev
+ * int64 [B][K]; `out` must not overlap `in`. */
+int asrk_reorder_rows(const void* in, const int64_t* parents, int B, int K, int64_t row_bytes, void* out, void* stream);
+
+/* Paged key/value cache in 8 bits: pages of 64 tokens, e4m3 values with one power of two per page, head and tensor.
+ * Sequence s is slot s * seq_stride of table / lens / starts, so that every K-th slot can be addressed as a cache of its
+ * own.  All pointers dev, owned by the caller:
+ *   kv      [num_layers][num_pages][kv_heads][2][64 * head_dim] bytes: keys [64][head_dim], values [head_dim][64]
+ *   exps    int8 [num_layers][num_pages][kv_heads][4]: exponent of the keys, of the values, 1 if the values hold a NaN, 0
+ *   table   int32 [slots][max_pages], -1 where there is no page;  lens, starts int32 [slots]: tokens now, and before the
+ *           last asrk_kv_extend;  refs int32 [num_pages]: sequences that hold the page (0: free)
+ *   status  int32 [2]: ASRK_KV_* bits of calls that could not be carried out (sticky); pages in use after a compaction
+ *   scratch asrk_kv_scratch_bytes(), zero before the first call
+ * head_dim 64 or 128.  kv, exps, refs, scratch 16-byte aligned. */
+#define ASRK_KV_PAGE 64
+enum { ASRK_KV_OUT_OF_PAGES = 1, ASRK_KV_TOO_LONG = 2, ASRK_KV_BAD_COUNT = 4, ASRK_KV_BAD_PARENT = 8 };
+typedef struct {
+    int num_layers, num_pages, kv_heads, head_dim, num_seqs, max_pages, seq_stride;
+    void* kv;
+    int8_t* exps;
+    int32_t *table, *lens, *starts, *refs, *status, *scratch;
+} asrk_kv_cache;
+
+size_t asrk_kv_scratch_bytes(int num_pages, int num_slots);
+
+/* Room for n_each[s] (dev int32 [num_seqs]; NULL: n_all each) more tokens: starts = lens, lens += n, the lowest free
+ * pages in the order of the sequences, and a copy of an open page that another sequence holds too (the first of its
+ * holders keeps it if all of them are extended).  All or nothing: if pages run out, or a count is negative or passes
+ * max_pages * 64, only starts = lens is done and `status` says why. */
+int asrk_kv_extend(const asrk_kv_cache* c, const int32_t* n_each, int n_all, void* stream);
+
+/* Sequence b K + k becomes what b K + parents[b][k] was, -1: empty (parents dev int64 [num_seqs / K][K], K <= 32).  No
+ * page is copied.  Any other value leaves the sequence as it was and sets ASRK_KV_BAD_PARENT. */
+int asrk_kv_reorder(const asrk_kv_cache* c, const int64_t* parents, int K, void* stream);
+
+/* Moves pages so that those in use are 0 .. status[1] - 1.  seq_stride must be 1. */
+int asrk_kv_compact(const asrk_kv_cache* c, void* stream);
+
+/* Rows 0 .. min(n, lens - starts) - 1 of k and v ([num_seqs][n][kv_heads][head_dim], ASRK_F32 | ASRK_BF16, strides in
+ * values, the last dimension dense, 16-byte aligned rows) become the tokens from starts[s] on of one layer. */
+int asrk_kv_write(const asrk_kv_cache* c, int layer, const void* k, const void* v, int dtype, int64_t seq_ld, int64_t row_ld,
+                  int64_t head_ld, int n, void* stream);
+
+/* Tokens first .. first + count - 1 of every sequence (first_each dev int32 [num_seqs], NULL: first_all) as bf16
+ * [layers][num_seqs][count][kv_heads][head_dim]; zeros where a sequence has no such token. */
+int asrk_kv_read(const asrk_kv_cache* c, int layer, int layers, const int32_t* first_each, int first_all, int count, void* k_out,
+                 void* v_out, void* stream);
+
+/* Attention over one layer of the cache: row i of sequence s, for i < lens - starts, sees tokens 0 .. starts[s] + i;
+ * the other rows become zero.  q bf16 [num_seqs][n][q_heads][head_dim] (strides in values, multiples of 8), q_heads a
+ * multiple of kv_heads, out bf16 [num_seqs][n][q_heads][head_dim] dense.  num_beams consecutive sequences are worked on
+ * together, and pages that their tables share are read once; it changes nothing else.  num_beams <= 32. */
+size_t asrk_kv_attention_workspace_bytes(const asrk_kv_cache* c, int n, int q_heads, int num_beams);
+int asrk_kv_attention(const asrk_kv_cache* c, int layer, const void* q, int64_t seq_ld, int64_t row_ld, int64_t head_ld, int n,
+                      int q_heads, int num_beams, float scale, void* out, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Measurement hook (no counterpart in the reference, which has no profiler: SURVEY section 5).
  * When enabled, every GEMM / attention / log-mel / LayerNorm launch is bracketed by HIP events on
  * its own stream; asrk_profile_read sums one category -- one per rocprof symbol: 0 gemm256p_kernel (persistent

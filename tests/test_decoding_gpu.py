@@ -1,0 +1,588 @@
+"""The decoding operators on the GPU against their 64-bit restatement (oracle/decoding.py).
+
+Tolerances.  What is held in the cache, and every whole number, is compared exactly.  Scores: a float32 sum of 32 exponentials
+per lane (32 * 2**-24), exponentials of a float32 argument (17 * 1.44 * 2**-24 for the terms that count) and a result of
+magnitude below 64 rounded to float32 (2**-19): together below 1e-5.  Attention: half a step of the bfloat16 result (2**-8 of
+it), the weights' rounding to 11 bits (2**-11 of sum p |v| / sum p), and float32 sums of products of up to 128 terms in the
+scores, a relative 128 * 2**-24 * sum |q k| * scale in the weights, below 2**-12 for the inputs here: 2**-10 for the two.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import decoding as od
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+# ---- selection
+
+
+def check_select(logits, scores, eos=None):
+    from asr_amd.decoding import beam_select
+
+    B, K = scores.shape
+    step = beam_select(logits, scores, eos)
+    want = od.select(logits.reshape(B, K, -1).double().cpu().numpy(), scores.double().cpu().numpy(), -1 if eos is None else eos)
+    got = [t.cpu().numpy() for t in step]
+    for i in (1, 2, 4, 5):
+        assert got[i].dtype == np.int64 and np.array_equal(got[i], want[i]), (i, got[i], want[i])
+    for i in (0, 3):
+        assert got[i].dtype == np.float32 and np.allclose(got[i], want[i], rtol=0, atol=1e-5), np.abs(got[i] - want[i]).max()
+    return step
+
+
+@pytest.mark.parametrize("B,K,V,dtype,pad", [
+    (1, 1, 2, "f32", 0), (2, 1, 3, "bf16", 0), (3, 2, 2, "f32", 1), (2, 16, 130, "f32", 0), (4, 8, 8192, "bf16", 0), (2, 3, 8193, "f32", 3),
+    (1, 5, 49157, "bf16", 59), (3, 5, 51865, "bf16", 0), (1, 16, 20001, "bf16", 0), (2, 7, 70001, "f32", 0), (130, 4, 97, "bf16", 0)])
+def test_select(B, K, V, dtype, pad):
+    g = _gen(B * 1000 + V)
+    x = (torch.randn((B * K, V + pad), generator=g, device="cuda") * 3).to(torch.bfloat16 if dtype == "bf16" else torch.float32)[:, :V]
+    s = -torch.rand((B, K), generator=g, device="cuda") * 20
+    check_select(x, s)
+    check_select(x, s, eos=int(x[0].argmax()))
+    if K > 1:
+        s[:, 1:] = -math.inf  # the first step
+        check_select(x, s, eos=V - 1)
+    if pad == 0:
+        check_select(x.view(B, K, V), s, eos=0)
+
+
+def test_select_last_position_of_a_run():
+    x = torch.randn((6, 4, 1001), generator=_gen(5), device="cuda")
+    check_select(x[:, -1], -torch.rand((2, 3), generator=_gen(6), device="cuda"))
+    check_select(x.view(2, 3, 4, 1001)[:, :, 2], -torch.rand((2, 3), generator=_gen(7), device="cuda"))
+
+
+@pytest.mark.parametrize("V", [40, 1024, 16385, 51865])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_select_ties_go_to_the_lowest_index(V, dtype):
+    K = 5
+    x = torch.zeros((2 * K, V), device="cuda", dtype=dtype)  # equal beams, equal words; odd rows start at odd addresses
+    check_select(x, torch.full((2, K), -3.0, device="cuda"))
+    x[:, 1::2] = -0.0  # equal to 0
+    check_select(x, torch.full((2, K), -3.0, device="cuda"), eos=0)
+    row = torch.randn((V,), generator=_gen(V), device="cuda").to(dtype)
+    row[V // 2:] = row[:V - V // 2].clone()  # every word twice
+    check_select(row.expand(2 * K, V).contiguous(), torch.full((2, K), -3.0, device="cuda"))
+    up = torch.arange(V, device="cuda").float().div(V).to(dtype)  # ascending: bf16 has long runs of equal values
+    check_select(torch.stack([up, up.flip(0)] * K), torch.linspace(-1, -7, 2 * K, device="cuda").view(2, K))
+
+
+def test_select_dead_beams():
+    g = _gen(11)
+    x = torch.randn((4, 4, 9001), generator=g, device="cuda")
+    s = -torch.rand((4, 4), generator=g, device="cuda")
+    x[0, 1, 17] = math.nan
+    x[0, 2, 8999] = math.inf
+    x[0, 3] = -math.inf
+    s[1, 0], s[1, 1], s[1, 2] = math.nan, math.inf, -math.inf
+    x[1, 2] = math.nan  # behind a dead score
+    s[2] = -math.inf  # nothing lives
+    x[3, :, 5:] = -math.inf  # fewer words than candidates
+    x[3, 0, :] = -math.inf
+    x[3, 0, 3] = 2.0
+    check_select(x.view(16, -1), s)
+    check_select(x.view(16, -1), s, eos=3)
+    check_select(x.view(16, -1).bfloat16(), s, eos=1)
+
+
+def test_reorder_states():
+    from asr_amd.decoding import reorder_states
+
+    g = _gen(3)
+    par = torch.randint(0, 5, (7, 5), generator=g, device="cuda")
+    for shape, dtype in (((7, 5, 3, 11), torch.int64), ((35, 13), torch.uint8), ((35,), torch.float32), ((7, 5, 4096), torch.bfloat16), ((35, 100000), torch.int16)):
+        x = torch.randint(0, 100, shape, generator=g, device="cuda").to(dtype)
+        want = x.reshape(7, 5, -1)[torch.arange(7, device="cuda")[:, None], par].reshape(shape)
+        assert torch.equal(reorder_states(x, par), want), (shape, dtype)
+    x = torch.randn((7, 5, 6), generator=g, device="cuda")
+    assert torch.equal(reorder_states(x.transpose(0, 1).contiguous().transpose(0, 1), par), x[torch.arange(7, device="cuda")[:, None], par])
+    par[2, 1], par[3, 4] = -1, 5  # no beams: the rows stay
+    y = reorder_states(x, par)
+    assert torch.equal(y[2, 1], x[2, 1]) and torch.equal(y[3, 4], x[3, 4]) and torch.equal(y[0], x[0, par[0]])
+
+
+# ---- the cache
+
+
+def both(num_seqs, max_len, heads, dim, layers=1, pages=None):
+    """A cache whose memory holds NaN bytes and wild exponents, and its restatement."""
+    from asr_amd.decoding import PagedKVCache
+
+    c = PagedKVCache(num_seqs, max_len, heads, dim, num_layers=layers, num_pages=pages)
+    c.kv.fill_(0x7F)
+    c.exps.fill_(77)
+    return c, od.Cache(num_seqs, max_len, heads, dim, layers, pages)
+
+
+def same_pages(c, o):
+    assert np.array_equal(c.table.cpu().numpy(), o.table)
+    assert np.array_equal(c.lens.cpu().numpy(), o.lens) and np.array_equal(c.starts.cpu().numpy(), o.starts)
+    assert np.array_equal(c.refs.cpu().numpy(), o.refs)
+    assert int(c.status[0]) == o.status
+
+
+def same_tokens(c, o, first, count, every=1):
+    view = c if every == 1 else c.leaders(every)
+    k, v = view.read(first, count)
+    f = first.cpu().numpy() if isinstance(first, torch.Tensor) else first
+    for layer in range(o.L):
+        for got, want in zip((k, v), o.read(f, count, layer, every)):
+            assert np.array_equal(got[layer].double().cpu().numpy(), want, equal_nan=True)
+        one = view.read(first, count, layer=layer)
+        assert torch.equal(one[0].nan_to_num(9), k[layer].nan_to_num(9)) and torch.equal(one[1].nan_to_num(9), v[layer].nan_to_num(9))
+
+
+def same_attention(c, o, q, layer=0, beams=1, every=1, scale=None, margins=None, name=""):
+    view = c if every == 1 else c.leaders(every)
+    got = view.attend(q, layer=layer, num_beams=beams, scale=scale).double().cpu().numpy()
+    x = q.double().cpu().numpy()
+    want, size = (o.attend(x, layer, scale, every, magnitude=m) for m in (False, True))
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    over = np.nan_to_num(np.abs(got - want) / (2.0 ** -8 * np.abs(want) + 2.0 ** -10 * size + 1e-30))
+    assert over.max() <= 1, (name, over.max(), np.unravel_index(over.argmax(), over.shape))
+    if margins is not None:
+        margins.add(f"cache attention {name} vs fp64", over.max(), 1.0, "of the bound")
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 200])
+def test_write_and_read(dim, dtype, n):
+    c, o = both(5, 500, 3, dim, layers=2)
+    g = _gen(n + dim)
+    for step, before in enumerate(([0, 0, 0, 0, 0], [1, 63, 64, 37, 0], [0, 5, 0, 64, 130])):  # pages opened at every offset
+        c.extend(torch.tensor(before, device="cuda"))
+        o.extend(before)
+        new = [n, max(0, n - 1), n, 1, (n + 1) // 2]
+        for count in (before, new):
+            if max(count) == 0:
+                continue
+            if count is new:
+                c.extend(torch.tensor(count, device="cuda", dtype=torch.int32))
+                o.extend(count)
+            k, v = (torch.randn((5, max(count), 3, dim), generator=g, device="cuda").to(dtype) * 2.0 ** (4 * step) for _ in range(2))
+            for layer in (1, 0):
+                c.write(k * (1 + layer), v, layer=layer)
+                o.write((k * (1 + layer)).double().cpu().numpy(), v.double().cpu().numpy(), layer)
+        same_pages(c, o)
+        same_tokens(c, o, 0, int(o.lens.max()) + 3)
+        same_tokens(c, o, c.starts, 70)
+        same_tokens(c, o, torch.tensor([0, 1, 63, 64, 499], device="cuda"), 1)
+
+
+def test_write_is_right_at_the_ends_of_the_range():
+    c, o = both(3, 200, 1, 64)
+    rows = torch.zeros((3, 70, 1, 64), device="cuda")
+    g = _gen(4)
+    rows[0] = torch.randn((70, 1, 64), generator=g, device="cuda") * 2.0 ** torch.randint(-140, 120, (70, 1, 64), generator=g, device="cuda").float()
+    rows[1, 0, 0, :8] = torch.tensor([3.4e38, -3.4e38, 1e-45, 1e38, math.inf, -math.inf, math.nan, 0.0])
+    rows[1, 64, 0, :4] = torch.tensor([448.0, 449.0, 17.0, 2.0 ** -70])
+    rows[2, 3, 0, 0] = 2.0 ** -80  # below the smallest exponent's smallest value
+    rows[2, 64, 0, 0] = math.nan
+    for n in (1, 5, 64):  # raises the exponents of open pages
+        c.extend(n)
+        o.extend(n)
+        k, v = rows[:, :n], rows[:, 70 - n:]
+        c.write(k, v)
+        o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+        same_tokens(c, o, 0, 70)
+
+
+def test_write_takes_any_strides():
+    c, o = both(2, 130, 2, 64)
+    g = _gen(8)
+    fused = torch.randn((2, 66, 8, 64), generator=g, device="cuda").bfloat16()
+    for k, v in ((fused[:, :, 4:6], fused[:, :, 6:]), (fused[:, :, 1:6:3], fused[:, :, 2:4]), (fused[:, :, :2].transpose(1, 2).contiguous().transpose(1, 2), fused[:, :, 6:]),
+                 (fused.view(-1)[1:1 + 66 * 2 * 64 * 2].view(2, 66, 2, 64), fused[:, :, 6:]), (fused[:1, :, :2].expand(2, 66, 2, 64), fused[:1, :, 2:4].expand(2, 66, 2, 64))):
+        c.reorder(torch.full((1, 2), -1, device="cuda"))
+        o.reorder([[-1, -1]])
+        c.extend(66)
+        o.extend(66)
+        c.write(k, v)
+        o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+        same_tokens(c, o, 0, 66)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_pages_over_a_random_life(seed):
+    """Prompts enter, are forked, grow, end and are compacted, in a pool that now and then is too small."""
+    rng = np.random.default_rng(seed)
+    B, K = [(2, 3), (3, 1), (1, 5), (4, 2)][seed]
+    c, o = both(B * K, 330, 2, 64, layers=2, pages=[16, 9, 14, 40][seed])
+    lead = c.leaders(K)
+
+    def put(cache, n, every):  # every token is written, in both layers
+        cache.extend(torch.from_numpy(n).cuda())
+        o.extend(n, every)
+        for layer in range(2):
+            k, v = (torch.from_numpy(rng.standard_normal((len(n), int(n.max()), 2, 64)) * 2.0 ** rng.integers(-3, 4)).float().cuda() for _ in range(2))
+            cache.write(k, v, layer=layer)
+            o.write(k.double().cpu().numpy(), v.double().cpu().numpy(), layer, every)
+
+    for step in range(40):
+        what = rng.integers(0, 6)
+        if what == 0:
+            put(lead, rng.integers(0, 150, B), K)
+        elif what == 1:
+            par = rng.integers(0, K, (B, K))
+            c.reorder(torch.from_numpy(par).cuda())
+            o.reorder(par)
+        elif what == 2:
+            par = np.where(rng.random((B, K)) < 0.4, -1, np.arange(K))
+            c.reorder(torch.from_numpy(par).cuda())
+            o.reorder(par)
+        elif what == 3:
+            used = c.compact()
+            assert int(used) == o.compact()
+        elif what == 4:
+            put(c, np.full(B * K, rng.integers(1, 70)), 1)
+        else:
+            put(c, rng.integers(0, 3, B * K), 1)
+        same_pages(c, o)
+        same_tokens(c, o, 0, 330)
+
+
+def test_what_does_not_fit_adds_nothing_and_is_reported():
+    from asr_amd import _lib
+
+    c, o = both(4, 256, 1, 64, pages=5)
+    c.extend(70)  # 8 pages
+    o.extend(70)
+    same_pages(c, o)
+    with pytest.raises(_lib.AsrkError, match="pages"):
+        c.check()
+    c.check()
+    o.status = 0
+    for n in ([64, 64, 64, 64], [1, 0, 0, 0], [1, 1, 0, 0], [200, 0, 0, 0], [-1, 0, 0, 0]):
+        c.extend(torch.tensor(n, device="cuda"))
+        o.extend(n)
+        same_pages(c, o)
+    with pytest.raises(_lib.AsrkError, match="pages.*max_len.*negative"):
+        c.check()
+    o.status = 0
+    c.reorder(torch.tensor([[1, 4], [-2, 0]], device="cuda"))
+    o.reorder([[1, 4], [-2, 0]])
+    same_pages(c, o)
+    with pytest.raises(_lib.AsrkError, match="parent"):
+        c.check()
+    k = torch.ones((4, 3, 1, 64), device="cuda")
+    c.write(k, k)  # no row is new
+    assert int((c.kv != 0x7F).sum()) == 0 and int((c.attend(k.bfloat16()) != 0).sum()) == 0
+
+
+def filled(rng, num_seqs, heads, dim, before, new, beams=1, shared=None, layers=1):
+    """Sequences of `before` tokens and `new` ones in both caches; groups of `beams` share their first `shared` tokens."""
+    before, new = np.asarray(before), np.asarray(new)
+    top = int((before + new).max()) + 1
+    c, o = both(num_seqs, top, heads, dim, layers, pages=num_seqs * (-(-top // 64)) + 3)
+    lead = c.leaders(beams)
+
+    def put(x, cache, every, n):
+        rows = int(max(n))
+        if rows == 0:
+            return
+        k, v = (torch.from_numpy(rng.standard_normal((len(n), rows, heads, dim)) * s).float().cuda() for s in (1.0, 1.5))
+        for layer in range(layers):
+            cache.write(k, v, layer=layer)
+            o.write(k.double().cpu().numpy(), v.double().cpu().numpy(), layer, every)
+
+    if beams > 1:
+        first = np.minimum(shared, before[::beams])
+        lead.extend(torch.from_numpy(first).cuda())
+        o.extend(first, beams)
+        put(None, lead, beams, first)
+        zero = np.zeros((num_seqs // beams, beams), np.int64)
+        c.reorder(torch.from_numpy(zero).cuda())
+        o.reorder(zero)
+        rest = before - np.repeat(first, beams)
+    else:
+        rest = before
+    for n in (rest, new):
+        c.extend(torch.from_numpy(n).cuda())
+        o.extend(n)
+        put(None, c, 1, n)
+    same_pages(c, o)
+    c.check()
+    return c, o
+
+
+@pytest.mark.parametrize("dim,heads,group", [(64, 5, 3), (64, 1, 8), (64, 2, 1), (128, 2, 4), (128, 1, 16), (128, 3, 7)])
+def test_attend_single_tokens(dim, heads, group, margins):
+    rng = np.random.default_rng(dim + group)
+    before = [0, 1, 62, 63, 64, 127, 300, 700]
+    c, o = filled(rng, 8, heads, dim, before, [1, 1, 1, 1, 1, 0, 1, 1])  # sequence 5 has ended
+    q = torch.from_numpy(rng.standard_normal((8, 1, heads * group, dim))).cuda().bfloat16() * 2
+    same_attention(c, o, q, margins=margins, name=f"1 token, d {dim}, {heads} x {group}")
+    assert int((c.attend(q)[5] != 0).sum()) == 0
+
+
+@pytest.mark.parametrize("dim,heads,group,n", [(64, 5, 3, 2), (64, 1, 1, 70), (128, 2, 2, 9), (64, 2, 3, 130), (128, 1, 4, 200), (128, 1, 17, 8), (64, 1, 128, 1)])
+def test_attend_several_tokens(dim, heads, group, n, margins):
+    """Prompts behind what is there: every row sees the tokens up to its own; short sequences leave rows empty."""
+    rng = np.random.default_rng(n)
+    c, o = filled(rng, 4, heads, dim, [0, 5, 64, 130], [n, max(0, n - 1), (n + 1) // 2, 0])
+    q = torch.from_numpy(rng.standard_normal((4, n, heads * group, dim))).cuda().bfloat16()
+    same_attention(c, o, q, margins=margins, name=f"{n} tokens, d {dim}, {heads} x {group}")
+    same_attention(c, o, q, scale=0.5, name="another scale")
+
+
+@pytest.mark.parametrize("dim,heads,group,beams,n", [(64, 5, 3, 5, 1), (128, 1, 4, 4, 1), (64, 1, 1, 32, 1), (64, 2, 2, 3, 3), (128, 2, 7, 5, 1), (64, 1, 8, 8, 2), (64, 1, 16, 4, 3)])
+def test_attend_beams(dim, heads, group, beams, n, margins):
+    """Beams that share all pages but the last, some, or none; num_beams says which are worked on together and nothing else."""
+    rng = np.random.default_rng(beams)
+    S = 3 * beams
+    before = np.repeat([260, 129, 64], beams) + rng.integers(0, 70, S) * np.repeat([0, 1, 0], beams)
+    new = rng.integers(0, n + 1, S)
+    new[:beams] = n
+    c, o = filled(rng, S, heads, dim, before, new, beams, np.array([250, 70, 64]))
+    q = torch.from_numpy(rng.standard_normal((S, n, heads * group, dim))).cuda().bfloat16()
+    same_attention(c, o, q, beams=beams, margins=margins, name=f"{beams} beams, d {dim}, {heads} x {group}, {n} tokens")
+    same_attention(c, o, q, beams=1, name="apart")
+    par = rng.integers(0, beams, (3, beams))  # pages shared in no order
+    c.reorder(torch.from_numpy(par).cuda())
+    o.reorder(par)
+    same_attention(c, o, q, beams=beams, name="reordered")
+
+
+@pytest.mark.parametrize("beams", [1, 3])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_keeps_nan_where_it_is_seen(beams, n):
+    """A NaN reaches the rows that see its token, and no others: not the earlier rows, not the other beams, not past the end."""
+    rng = np.random.default_rng(7)
+    S = 2 * beams
+    c, o = filled(rng, S, 1, 64, [100] * S, [n] * S, beams, np.array([90, 64]))
+    k, v = (torch.from_numpy(rng.standard_normal((S, n, 1, 64))).float().cuda() for _ in range(2))
+    v[1, n // 2, 0, 5] = math.inf
+    v[0, n - 1, 0, 63] = math.nan
+    k[S - 1, n - 1, 0, 0] = math.nan
+    c.write(k, v)
+    o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+    q = torch.from_numpy(rng.standard_normal((S, n, 3, 64))).cuda().bfloat16()
+    same_attention(c, o, q, beams=beams)
+    assert bool(c.attend(q, num_beams=beams).isnan().any()) and not bool(c.attend(q, num_beams=beams).isnan().all())
+
+
+def test_attend_over_pages_of_very_different_scales():
+    """Values of 2**-60 next to values of 2**60: each row is right to its own size where the weights say so."""
+    rng = np.random.default_rng(9)
+    c, o = both(2, 320, 1, 64)
+    for e in (-50.0, 3.0, -9.0, 60.0):
+        c.extend(64)
+        o.extend(64)
+        k = torch.from_numpy(rng.standard_normal((2, 64, 1, 64))).float().cuda()
+        v = torch.from_numpy(rng.standard_normal((2, 64, 1, 64))).float().cuda() * 2.0 ** e
+        c.write(k, v)
+        o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+        q = torch.from_numpy(rng.standard_normal((2, 64, 2, 64))).cuda().bfloat16()
+        same_attention(c, o, q)
+        same_attention(c, o, q[:, :1])
+
+
+def test_attend_takes_any_strides():
+    rng = np.random.default_rng(10)
+    c, o = filled(rng, 3, 2, 64, [70, 3, 100], [2, 2, 2], layers=2)
+    fused = torch.from_numpy(rng.standard_normal((3, 5, 14, 64))).cuda().bfloat16()
+    for q in (fused[:, :2, :6], fused[:, 3:, 8:], fused[:, ::4, 1:13:2], fused.transpose(1, 2)[:, 4:6, :4].contiguous(), fused.view(-1)[3:3 + 3 * 2 * 4 * 64].view(3, 2, 4, 64),
+              fused[:1, :2, :4].expand(3, 2, 4, 64)):
+        same_attention(c, o, q, layer=1)
+
+
+def test_leaders_view_reads_and_attends():
+    rng = np.random.default_rng(12)
+    c, o = filled(rng, 6, 1, 128, [40, 9, 9, 90, 9, 9], [3, 1, 1, 3, 1, 1])
+    q = torch.from_numpy(rng.standard_normal((2, 3, 2, 128))).cuda().bfloat16()
+    same_attention(c, o, q, every=3)
+    same_tokens(c, o, 30, 70, every=3)
+
+
+def test_offsets_pass_32_bits():
+    """Two layers of 300000 pages of 16 KiB: the pages in use lie beyond 8 GiB."""
+    from asr_amd.decoding import PagedKVCache
+
+    P = 300000
+    c = PagedKVCache(2, 256, 1, 128, num_layers=2, num_pages=P)
+    o = od.Cache(2, 256, 1, 128, 2, 8)
+    c.refs[:P - 8] = 1  # held by others
+    c.extend(130)
+    o.extend(130)
+    assert np.array_equal(c.table.cpu().numpy(), np.where(o.table >= 0, o.table + P - 8, -1))
+    g = _gen(2)
+    k, v = (torch.randn((2, 130, 1, 128), generator=g, device="cuda") for _ in range(2))
+    c.write(k, v, layer=1)
+    o.write(k.double().cpu().numpy(), v.double().cpu().numpy(), 1)
+    same_tokens(c, o, 0, 140)
+    same_attention(c, o, torch.randn((2, 1, 4, 128), generator=g, device="cuda").bfloat16(), layer=1)
+    c.refs[:P - 8] = 0
+    assert int(c.compact()) == 6 and int(c.table.max()) == 5
+    same_tokens(c, o, 0, 140)
+
+
+def test_refusals():
+    from asr_amd import _lib
+    from asr_amd.decoding import PagedKVCache, beam_select, reorder_states
+
+    c = PagedKVCache(4, 100, 2, 64, num_layers=2)
+    ok = torch.zeros((4, 1, 2, 64), device="cuda", dtype=torch.bfloat16)
+    for k, v in ((ok[:3], ok[:3]), (ok, ok[:, :, :1]), (ok.half(), ok.half()), (ok, ok.float()), (ok[0], ok[0]), (ok[..., :32], ok[..., :32])):
+        with pytest.raises(ValueError):
+            c.write(k, v)
+    for q, kw in ((ok[:3], {}), (ok.float(), {}), (ok[:, :, :1], {}), (ok[..., :32], {}), (ok, dict(num_beams=3)), (ok, dict(num_beams=0)), (ok, dict(layer=2)),
+                  (ok, dict(layer=-1)), (ok[:, :, :0], {})):
+        with pytest.raises(ValueError):
+            c.attend(q, **kw)
+    with pytest.raises(ValueError):
+        c.attend(ok.clone().requires_grad_())
+    with pytest.raises(ValueError):
+        beam_select(torch.zeros((4, 9), device="cuda", requires_grad=True), torch.zeros((2, 2), device="cuda"))
+    for n in (-1, 129, torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(4, device="cuda"), torch.zeros((4, 1), dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError):
+            c.extend(n)
+    for p in (torch.zeros((2, 2), dtype=torch.int32, device="cuda"), torch.zeros((2, 3), dtype=torch.int64, device="cuda"), torch.zeros((4,), dtype=torch.int64, device="cuda")):
+        with pytest.raises(ValueError):
+            c.reorder(p)
+    for bad in (lambda: c.read(-1, 3), lambda: c.read(0, -1), lambda: c.read(0, 3, layer=2), lambda: c.read(torch.zeros(3, dtype=torch.int32, device="cuda"), 3),
+                lambda: c.leaders(3), lambda: c.leaders(0), lambda: c.leaders(2).compact()):
+        with pytest.raises(ValueError):
+            bad()
+    for cpu in (lambda: c.write(ok.cpu(), ok.cpu()), lambda: c.attend(ok.cpu()), lambda: c.extend(torch.zeros(4, dtype=torch.int32)), lambda: c.reorder(torch.zeros((2, 2), dtype=torch.int64))):
+        with pytest.raises(_lib.AsrkError):
+            cpu()
+    with pytest.raises(ValueError):
+        reorder_states(ok.cpu(), torch.zeros((2, 2), dtype=torch.int64, device="cuda")) if False else reorder_states(ok[:3], torch.zeros((2, 2), dtype=torch.int64, device="cuda"))
+    assert tuple(c.attend(ok[:, :0]).shape) == (4, 0, 2, 64)
+    c.write(ok[:, :0], ok[:, :0])
+    assert tuple(c.read(0, 0)[0].shape) == (2, 4, 0, 2, 64)
+    assert beam_select(torch.zeros((0, 9), device="cuda"), torch.zeros((0, 2), device="cuda")).tokens.shape == (0, 2)
+    assert int(c.status[0]) == 0 and int(c.lens.sum()) == 0
+
+
+# ---- together
+
+
+def _step(c, logits, scores, history, k, v, q, beams, eos):
+    from asr_amd.decoding import beam_select, reorder_states
+
+    step = beam_select(logits, scores, eos)
+    c.reorder(step.parents)
+    history.copy_(reorder_states(history, step.parents))
+    c.extend(1)
+    for layer in range(c.num_layers):
+        c.write(k[layer], v[layer], layer=layer)
+    out = torch.stack([c.attend(q[layer], layer=layer, num_beams=beams) for layer in range(c.num_layers)])
+    scores.copy_(step.scores)
+    return out, step.tokens
+
+
+def _prompted(seed, B, K, heads, dim, layers, prompt, max_len):
+    from asr_amd.decoding import PagedKVCache
+
+    g = _gen(seed)
+    c = PagedKVCache(B * K, max_len, heads, dim, num_layers=layers)
+    lead = c.leaders(K)
+    lead.extend(torch.tensor([prompt - i for i in range(B)], device="cuda"))
+    for layer in range(layers):
+        k, v = (torch.randn((B, prompt, heads, dim), generator=g, device="cuda").bfloat16() for _ in range(2))
+        lead.write(k, v, layer=layer)
+    c.reorder(torch.zeros((B, K), dtype=torch.int64, device="cuda"))
+    return c
+
+
+def _inputs(seed, B, K, heads, group, dim, layers, V):
+    g = _gen(seed)
+    return dict(logits=torch.randn((B * K, V), generator=g, device="cuda") * 3,
+                k=torch.randn((layers, B * K, 1, heads, dim), generator=g, device="cuda").bfloat16(),
+                v=torch.randn((layers, B * K, 1, heads, dim), generator=g, device="cuda").bfloat16(),
+                q=torch.randn((layers, B * K, 1, heads * group, dim), generator=g, device="cuda").bfloat16())
+
+
+def test_steps_together_follow_the_oracle():
+    B, K, heads, group, dim, V = 2, 3, 2, 2, 64, 57
+    c, o = both(B * K, 200, heads, dim)
+    rng = np.random.default_rng(21)
+    n = np.array([70, 61])
+    c.leaders(K).extend(torch.from_numpy(n).cuda())
+    o.extend(n, K)
+    k, v = (torch.from_numpy(rng.standard_normal((B, 70, heads, dim))).float().cuda() for _ in range(2))
+    c.leaders(K).write(k, v)
+    o.write(k.double().cpu().numpy(), v.double().cpu().numpy(), every=K)
+    zero = np.zeros((B, K), np.int64)
+    c.reorder(torch.from_numpy(zero).cuda())
+    o.reorder(zero)
+    scores = torch.zeros((B, K), device="cuda")
+    scores[:, 1:] = -math.inf
+    for t in range(12):
+        x = _inputs(100 + t, B, K, heads, group, dim, 1, V)
+        step = check_select(x["logits"], scores, eos=5)
+        c.reorder(step.parents)
+        o.reorder(step.parents.cpu().numpy())
+        c.extend(1)
+        o.extend(1)
+        c.write(x["k"][0], x["v"][0])
+        o.write(x["k"][0].double().cpu().numpy(), x["v"][0].double().cpu().numpy())
+        same_pages(c, o)
+        same_attention(c, o, x["q"][0], beams=K)
+        scores = step.scores
+    same_tokens(c, o, 0, 90)
+
+
+def test_a_captured_step_replays_like_the_eager_one():
+    B, K, heads, group, dim, layers, V = 2, 4, 2, 3, 64, 2, 4099
+    args = (31, B, K, heads, dim, layers, 90, 200)
+    eager, graphed = _prompted(*args), _prompted(*args)
+    state = {}
+    for name in ("eager", "graphed"):
+        s = torch.zeros((B, K), device="cuda")
+        s[:, 1:] = -math.inf
+        state[name] = dict(scores=s, history=torch.arange(B * K * 7, device="cuda").view(B, K, 7))
+    x = _inputs(1, B, K, heads, group, dim, layers, V)
+    warm = _prompted(*args)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        _step(warm, **{n: t.clone() for n, t in x.items()}, beams=K, eos=7, **{n: t.clone() for n, t in state["eager"].items()})
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _step(graphed, **x, beams=K, eos=7, **state["graphed"])
+    for t in range(80):  # over the end of a page and of max_len's table
+        fresh = _inputs(200 + t, B, K, heads, group, dim, layers, V)
+        for n, tensor in fresh.items():
+            x[n].copy_(tensor)
+        graph.replay()
+        want = _step(eager, **fresh, beams=K, eos=7, **state["eager"])
+        if t % 9 == 0:
+            torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), t
+        for n in ("table", "lens", "starts", "refs", "kv", "exps"):
+            assert torch.equal(getattr(eager, n), getattr(graphed, n)), (t, n)
+        assert torch.equal(state["eager"]["scores"], state["graphed"]["scores"]) and torch.equal(state["eager"]["history"], state["graphed"]["history"])
+    assert int(eager.lens.max()) == 170
+    eager.check()
+
+
+def test_two_caches_on_two_streams():
+    args = (41, 2, 5, 1, 64, 1, 130, 300)
+    want = _prompted(*args)
+    outs = []
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    caches = [_prompted(*args) for _ in range(2)]
+    torch.cuda.synchronize()
+    scores = [torch.zeros((2, 5), device="cuda") for _ in range(3)]
+    hist = [torch.zeros((2, 5, 3), device="cuda", dtype=torch.int64) for _ in range(3)]
+    xs = [_inputs(300 + t, 2, 5, 1, 3, 64, 1, 9001) for t in range(10)]
+    torch.cuda.synchronize()
+    for t in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs.append(_step(caches[i], **xs[t], beams=5, eos=3, scores=scores[i], history=hist[i])[0])
+    ref = [_step(want, **xs[t], beams=5, eos=3, scores=scores[2], history=hist[2])[0] for t in range(10)]
+    torch.cuda.synchronize()
+    for t in range(10):
+        assert torch.equal(outs[2 * t], ref[t]) and torch.equal(outs[2 * t + 1], ref[t])

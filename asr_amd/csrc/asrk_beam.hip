@@ -55,104 +55,126 @@ struct SelVec<bf16_t> {
     }
 };
 
-// One workgroup per (chunk, row).  Keys are (value, ~index) in 64 bits and hence all different, which bounds the work
-// for any input: the n-th largest of the 64 lane maxima of a wave is a lower bound of its n-th largest key, and only
-// the n lanes at or above it can hold keys that count, so at most 32 n keys per wave reach LDS (with random logits
-// about 1.5 n do).
+constexpr int sel_lanes(int n) { return n + 8; }  // lanes of a workgroup whose values may be candidates
+
+// One workgroup per (chunk, row).  A threshold with at least n of the 256 lane maxima at or above it is a lower bound of
+// the chunk's n-th best value, and only those lanes can hold values that count.  Bisection finds one with n .. n + 8 such
+// lanes in a few steps, a compare and a bit count per wave's worth of lanes; every wave does it for itself on all 256.
+// Where equal values leave no such threshold it falls back to ranking the lane maxima by (value, ~word), which are all
+// different.  Either way at most sel_lanes(n) lanes of 32 keys reach LDS, for any input (with random logits about n + 6
+// keys do).
 template <class T>
 __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ logits, int64_t ld, int V, int n,
                                                          uint64_t* __restrict__ keys, float2* __restrict__ stats) {
     constexpr int VEC = SelVec<T>::N;
-    __shared__ uint64_t cand[SEL_WAVES][SEL_MAX_N * SEL_EPT];
-    __shared__ int count[SEL_WAVES];
+    extern __shared__ uint64_t cand[];  // [sel_lanes(n) * SEL_EPT]
+    __shared__ __attribute__((aligned(16))) uint32_t bests[256];
+    __shared__ uint32_t firsts[256];
+    __shared__ int count;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = blockIdx.y, chunk = blockIdx.x;
     const T* p = logits + (int64_t)row * ld;
+    const int e0 = (chunk * SEL_WAVES + wave) * 64 * SEL_EPT + lane * VEC;  // word of slot 0; slot s: word(s), ascending
+    auto word = [&](int s) __attribute__((always_inline)) { return e0 + s / VEC * 64 * VEC + s % VEC; };
     float x[SEL_EPT];
-    int first[SEL_EPT / VEC];
-#pragma unroll
-    for (int j = 0; j < SEL_EPT / VEC; ++j) {
-        const int e = (chunk * SEL_WAVES + wave) * 64 * SEL_EPT + (j * 64 + lane) * VEC;
-        first[j] = e;
-        if (e + VEC <= V) {
-            SelVec<T>::unpack(*reinterpret_cast<const typename SelVec<T>::Raw*>(p + e), x + j * VEC);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) x[j * VEC + i] = e + i < V ? (float)p[e + i] : NEG_INF;
-        }
-    }
-    float top = NEG_INF;
-    bool bad = false;
-    uint64_t best = 0;
-    auto key = [&](int j, int i) __attribute__((always_inline)) -> uint64_t {
-        const int e = first[j] + i;
-        return e < V ? ((uint64_t)ord32(x[j * VEC + i]) << 32) | (0xffffffffu - (uint32_t)e) : 0;
-    };
-#pragma unroll
-    for (int j = 0; j < SEL_EPT / VEC; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float& v = x[j * VEC + i];
-            bad |= !(v < __builtin_inff());
-            v = v + 0.0f;
-            top = fmaxf(top, v);
-            const uint64_t k = key(j, i);
-            best = k > best ? k : best;
-        }
-    top = wave_max(top);
-    float sum = 0.f;
-    if (top > NEG_INF) {
-#pragma unroll
-        for (int i = 0; i < SEL_EPT; ++i) sum += __builtin_amdgcn_exp2f((x[i] - top) * 1.4426950408889634f);
-    }
-    sum = wave_sum(sum);
-    bad = __any(bad);
-    if (lane == 0)
-        stats[((int64_t)row * gridDim.x + chunk) * SEL_WAVES + wave] = make_float2(bad ? __builtin_inff() : top, sum);
-
-    // the wave's threshold: the lane maximum of rank n - 1
-    int rank = 0;
-    const uint32_t bh = (uint32_t)(best >> 32), bl = (uint32_t)best;
-#pragma unroll 8
-    for (int l = 0; l < 64; ++l) {
-        const uint64_t o = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(bh, l) << 32) | (uint32_t)__builtin_amdgcn_readlane(bl, l);
-        rank += o > best ? 1 : 0;
-    }
-    const uint64_t at = __ballot(rank == n - 1 && best != 0);
-    uint64_t tau = 1;  // fewer than n lanes hold anything: all of it counts
-    if (at) {
-        const int l = __builtin_ctzll(at);
-        tau = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(bh, l) << 32) | (uint32_t)__builtin_amdgcn_readlane(bl, l);
-    }
-    int c = 0;
-    if (__any(best >= tau)) {
+    if (e0 + (SEL_EPT / VEC - 1) * 64 * VEC + VEC <= V) {
 #pragma unroll
         for (int j = 0; j < SEL_EPT / VEC; ++j)
+            SelVec<T>::unpack(*reinterpret_cast<const typename SelVec<T>::Raw*>(p + word(j * VEC)), x + j * VEC);
+    } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const uint64_t k = key(j, i);
-                const uint64_t m = __ballot(k >= tau);
+        for (int j = 0; j < SEL_EPT / VEC; ++j) {
+            if (word(j * VEC) + VEC <= V) {
+                SelVec<T>::unpack(*reinterpret_cast<const typename SelVec<T>::Raw*>(p + word(j * VEC)), x + j * VEC);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[j * VEC + i] = word(j * VEC + i) < V ? (float)p[word(j * VEC + i)] : NEG_INF;
+            }
+        }
+    }
+    float best = NEG_INF;
+#pragma unroll
+    for (int s = 0; s < SEL_EPT; ++s) best = fmaxf(best, x[s]);
+    // the lane maxima of all four waves, lane l of wave w at 4 l + w; 0: no word at all
+    bests[lane * 4 + wave] = e0 < V ? ord32(best + 0.0f) : 0;  // -0 counts as 0
+    if (threadIdx.x == 0) count = 0;
+    const float top = wave_max(best);
+    const float ref = top > NEG_INF ? top : 0.f;
+    float sum = 0.f;  // NaN if one of the logits is
+#pragma unroll
+    for (int s = 0; s < SEL_EPT; ++s) sum += __builtin_amdgcn_exp2f((x[s] - ref) * 1.4426950408889634f);
+    sum = wave_sum(sum);
+    if (lane == 0)
+        stats[((int64_t)row * gridDim.x + chunk) * SEL_WAVES + wave] = make_float2(sum == sum ? top : __builtin_inff(), sum);
+    __syncthreads();
+
+    constexpr uint32_t LOWEST = 0x007fffffu;  // -inf
+    const u32x4 mine = *reinterpret_cast<const u32x4*>(bests + lane * 4);
+    auto at_least = [&](uint32_t t) __attribute__((always_inline)) {
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) c += __popcll(__ballot(mine[w] >= t));
+        return c;
+    };
+    uint32_t tau = LOWEST, tau_low = 0;  // n lanes or fewer hold anything: all of it counts
+    if (at_least(1) > n) {
+        uint32_t lo = LOWEST, hi = 0xff800001u;  // at or above lo: too many; hi: too few (above +inf)
+        bool found = false;
+        {  // most lane maxima lie within a few units below the largest
+            float m = wave_max(fmaxf(fmaxf(unord32(mine[0] ? mine[0] : LOWEST), unord32(mine[1] ? mine[1] : LOWEST)),
+                                     fmaxf(unord32(mine[2] ? mine[2] : LOWEST), unord32(mine[3] ? mine[3] : LOWEST))));
+            hi = __builtin_amdgcn_readfirstlane(ord32(m)) + 1;
+        }
+        while (!found && hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int c = at_least(mid);
+            found = c >= n && c <= sel_lanes(n);
+            if (found) tau = mid;
+            else if (c < n) hi = mid;
+            else lo = mid;
+        }
+        if (!found) {  // the n-th lane by (value, ~word)
+            uint32_t first = 0;
+#pragma unroll
+            for (int s = SEL_EPT - 1; s >= 0; --s) first = x[s] == best ? 0xffffffffu - (uint32_t)word(s) : first;
+            firsts[lane * 4 + wave] = first;
+            __syncthreads();  // every wave is here: they all look at the same 256 values
+            for (int w = 0; w < 4; ++w) {
+                const uint64_t key = ((uint64_t)bests[lane * 4 + w] << 32) | firsts[lane * 4 + w];
+                int rank = 0;
+#pragma unroll 4
+                for (int l = 0; l < 256; ++l) rank += (((uint64_t)bests[l] << 32) | firsts[l]) > key ? 1 : 0;
+                const uint64_t m = __ballot(rank == n - 1 && key >> 32);
                 if (m) {
-                    if (k >= tau) cand[wave][c + __popcll(m & ((1ull << lane) - 1))] = k;
-                    c += __popcll(m);
+                    tau = __builtin_amdgcn_readlane((uint32_t)(key >> 32), __builtin_ctzll(m));
+                    tau_low = __builtin_amdgcn_readlane((uint32_t)key, __builtin_ctzll(m));
                 }
             }
+        }
     }
-    if (lane == 0) count[wave] = c;
+    const float least = unord32(tau);
+    if (__any(best >= least)) {
+#pragma unroll
+        for (int s = 0; s < SEL_EPT; ++s) {
+            if (!__any(x[s] >= least)) continue;
+            const uint32_t high = ord32(x[s] + 0.0f), low = 0xffffffffu - (uint32_t)word(s);
+            if (x[s] >= least && word(s) < V && (high > tau || low >= tau_low)) cand[atomicAdd(&count, 1)] = ((uint64_t)high << 32) | low;
+        }
+    }
     __syncthreads();
     uint64_t* out = keys + ((int64_t)row * gridDim.x + chunk) * n;
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < SEL_WAVES; ++w) total += count[w];
+    const int total = count;
     for (int r = total + (int)threadIdx.x; r < n; r += 256) out[r] = 0;
-    for (int w = 0; w < SEL_WAVES; ++w)
-        for (int t = threadIdx.x; t < count[w]; t += 256) {
-            const uint64_t mine = cand[w][t];
-            int r = 0;
-            for (int w2 = 0; w2 < SEL_WAVES; ++w2)
-                for (int u = 0; u < count[w2]; ++u) r += cand[w2][u] > mine ? 1 : 0;
-            if (r < n) out[r] = mine;
-        }
+    const int part = threadIdx.x & 3;  // four threads per key, each against a quarter of them
+    for (int t = threadIdx.x >> 2; t < (total + 63) / 64 * 64; t += 64) {
+        const uint64_t key = t < total ? cand[t] : 0;
+        int r = 0;
+#pragma unroll 4
+        for (int u = part; u < total; u += 4) r += cand[u] > key ? 1 : 0;
+        r += __shfl_xor(r, 1, 64);
+        r += __shfl_xor(r, 2, 64);
+        if (part == 0 && t < total && r < n) out[r] = key;
+    }
 }
 
 struct Pick {
@@ -163,13 +185,16 @@ __device__ __forceinline__ bool ahead(const Pick& a, const Pick& b) { return a.v
 
 // One workgroup per utterance: the row sums in 64 bits, then the best n of the chunks' sorted lists.  Values are
 // compared in 64 bits, where different logits of a beam stay different (and equal ones equal); the n-th best list head
-// bounds the n-th best value from below, so at most n lists of at most n keys are looked at.
-__global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restrict__ keys, const float2* __restrict__ stats,
-                                                        const float* __restrict__ scores, int K, int V, int chunks, int n,
-                                                        int64_t eos, float* __restrict__ out_scores,
-                                                        int64_t* __restrict__ out_tokens, int64_t* __restrict__ out_parents,
-                                                        float* __restrict__ cand_scores, int64_t* __restrict__ cand_tokens,
-                                                        int64_t* __restrict__ cand_parents) {
+// bounds the n-th best value from below, so at most n lists of at most n keys are candidates.  Bound by its chain of
+// dependent steps: everything it may need is loaded first (a load is about a microsecond, the arithmetic is less).
+constexpr int JOIN_T = 512;
+constexpr int JOIN_HELD = 4;  // keys per thread that are loaded ahead: all of them up to 2048
+__global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __restrict__ keys, const float2* __restrict__ stats,
+                                                           const float* __restrict__ scores, int K, int V, int chunks, int n,
+                                                           int64_t eos, float* __restrict__ out_scores,
+                                                           int64_t* __restrict__ out_tokens, int64_t* __restrict__ out_parents,
+                                                           float* __restrict__ cand_scores, int64_t* __restrict__ cand_tokens,
+                                                           int64_t* __restrict__ cand_parents) {
     __shared__ double lse[SEL_MAX_BEAMS];
     __shared__ double score[SEL_MAX_BEAMS];
     __shared__ int alive[SEL_MAX_BEAMS];
@@ -183,78 +208,99 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const uint64_t* __restri
     __shared__ uint32_t best_at[SEL_MAX_N];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = blockIdx.x;
+    const int lists = K * chunks, all = lists * n;
+    const uint64_t* mine = keys + (int64_t)b * all;
+    uint64_t held[JOIN_HELD];
+#pragma unroll
+    for (int q = 0; q < JOIN_HELD; ++q) {
+        const int i = q * JOIN_T + threadIdx.x;
+        held[q] = i < all ? mine[i] : 0;
+    }
     if (threadIdx.x == 0) {
         n_cand = 0;
         tau = Pick{-__builtin_inf(), 0xffffffffu};  // everything is ahead of it
     }
-    for (int k = wave; k < K; k += 4) {
+    for (int k = wave; k < K; k += JOIN_T / 64) {
         const float2* st = stats + ((int64_t)b * K + k) * chunks * SEL_WAVES;
-        float top = NEG_INF;
-        for (int i = lane; i < chunks * SEL_WAVES; i += 64) top = fmaxf(top, st[i].x);
+        const float s = scores[(int64_t)b * K + k];
+        const float2 first = lane < chunks * SEL_WAVES ? st[lane] : make_float2(NEG_INF, 0.f);
+        float top = first.x;
+        for (int i = lane + 64; i < chunks * SEL_WAVES; i += 64) top = fmaxf(top, st[i].x);
         top = wave_max(top);
-        double sum = 0.0;
         const bool ok = top > NEG_INF && top < __builtin_inff();
-        if (ok)
-            for (int i = lane; i < chunks * SEL_WAVES; i += 64)
+        double sum = 0.0;
+        if (ok) {
+            if (first.x > NEG_INF) sum = (double)first.y * exp((double)first.x - (double)top);
+            for (int i = lane + 64; i < chunks * SEL_WAVES; i += 64)
                 if (st[i].x > NEG_INF) sum += (double)st[i].y * exp((double)st[i].x - (double)top);
+        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
         if (lane == 0) {
-            const float s = scores[(int64_t)b * K + k];
             alive[k] = ok && s > NEG_INF && s < __builtin_inff();
             lse[k] = ok ? (double)top + log(sum) : 0.0;
             score[k] = (double)s;
         }
     }
     __syncthreads();
-    const int lists = K * chunks;
-    // entry j of list l; false: none
-    auto entry = [&](int l, int j, Pick& p) -> bool {
-        const int k = l / chunks, c = l - k * chunks;
+    // entry j of list l, whose key is `key`; false: none
+    auto entry = [&](int l, int j, uint64_t key, Pick& p) -> bool {
+        const int k = l / chunks;
         if (!alive[k]) {  // a dead beam: its words in order
             p = Pick{-__builtin_inf(), (uint32_t)(k * V + j)};
-            return c == 0 && j < V;
+            return l == k * chunks && j < V;
         }
-        const uint64_t key = keys[(((int64_t)b * K + k) * chunks + c) * n + j];
         p = Pick{score[k] + ((double)unord32((uint32_t)(key >> 32)) - lse[k]), (uint32_t)(k * V) + (0xffffffffu - (uint32_t)key)};
         return key != 0;
     };
-    for (int l = threadIdx.x; l < lists; l += 256) {
+    auto each = [&](auto&& f) __attribute__((always_inline)) {  // f(list, place in it, key)
+#pragma unroll
+        for (int q = 0; q < JOIN_HELD; ++q) {
+            const int i = q * JOIN_T + threadIdx.x;
+            if (i < all) f(i / n, i % n, held[q]);
+        }
+        for (int i = JOIN_HELD * JOIN_T + threadIdx.x; i < all; i += JOIN_T) f(i / n, i % n, mine[i]);
+    };
+    each([&](int l, int j, uint64_t key) {
+        if (j) return;
         Pick p;
-        const bool any = entry(l, 0, p);
+        const bool any = entry(l, 0, key, p);
         head_v[l] = any ? p.v : __builtin_nan("");
         head_at[l] = any ? p.at : 0xffffffffu;
-    }
+    });
     __syncthreads();
-    for (int l = threadIdx.x; l < lists; l += 256) {
-        const Pick mine{head_v[l], head_at[l]};
-        if (mine.v != mine.v) continue;
+    const int part = threadIdx.x & 3;  // four threads per head, and per candidate, each against a quarter of the others
+    for (int l = threadIdx.x >> 2; l < lists; l += JOIN_T / 4) {
+        const Pick p{head_v[l], head_at[l]};
         int r = 0;
-        for (int u = 0; u < lists; ++u) r += ahead(Pick{head_v[u], head_at[u]}, mine) ? 1 : 0;  // NaN is ahead of nothing
-        if (r == n - 1) tau = mine;
+#pragma unroll 4
+        for (int u = part; u < lists; u += 4) r += ahead(Pick{head_v[u], head_at[u]}, p) ? 1 : 0;  // NaN is ahead of nothing
+        r += __shfl_xor(r, 1, 64);
+        r += __shfl_xor(r, 2, 64);
+        if (part == 0 && r == n - 1 && p.v == p.v) tau = p;
     }
     __syncthreads();
     const Pick least = tau;
-    for (int l = threadIdx.x; l < lists; l += 256) {
-        Pick p{head_v[l], head_at[l]};
-        if (p.v != p.v) continue;
-        for (int j = 0; j < n; ++j) {
-            if (j > 0 && !entry(l, j, p)) break;
-            if (ahead(least, p)) break;  // lists are sorted
-            const int at = atomicAdd(&n_cand, 1);
-            cand_v[at] = p.v;
-            cand_at[at] = p.at;
-        }
-    }
+    each([&](int l, int j, uint64_t key) {
+        if (head_v[l] != head_v[l] || ahead(least, Pick{head_v[l], head_at[l]})) return;
+        Pick p;
+        if (!entry(l, j, key, p) || ahead(least, p)) return;
+        const int at = atomicAdd(&n_cand, 1);
+        cand_v[at] = p.v;
+        cand_at[at] = p.at;
+    });
     __syncthreads();
     const int c = n_cand;
-    for (int t = threadIdx.x; t < c; t += 256) {
-        const Pick mine{cand_v[t], cand_at[t]};
+    for (int t = threadIdx.x >> 2; t < c; t += JOIN_T / 4) {
+        const Pick p{cand_v[t], cand_at[t]};
         int r = 0;
-        for (int u = 0; u < c; ++u) r += ahead(Pick{cand_v[u], cand_at[u]}, mine) ? 1 : 0;
-        if (r < n) {
-            best_v[r] = mine.v;
-            best_at[r] = mine.at;
+#pragma unroll 4
+        for (int u = part; u < c; u += 4) r += ahead(Pick{cand_v[u], cand_at[u]}, p) ? 1 : 0;
+        r += __shfl_xor(r, 1, 64);
+        r += __shfl_xor(r, 2, 64);
+        if (part == 0 && r < n) {
+            best_v[r] = p.v;
+            best_at[r] = p.at;
         }
     }
     __syncthreads();
@@ -317,13 +363,14 @@ extern "C" int asrk_beam_select(const void* logits, int dtype, int64_t ld, const
     uint64_t* keys = (uint64_t*)ws;
     float2* stats = (float2*)(keys + (size_t)B * K * chunks * 2 * K);
     hipStream_t st = (hipStream_t)stream;
+    const size_t lds = (size_t)sel_lanes(2 * K) * SEL_EPT * sizeof(uint64_t);  // 10 KiB at most
     if (dtype == ASRK_F32)
-        hipLaunchKernelGGL(beam_chunk_kernel<float>, dim3(chunks, B * K), dim3(256), 0, st, (const float*)logits, ld, V, 2 * K, keys,
+        hipLaunchKernelGGL(beam_chunk_kernel<float>, dim3(chunks, B * K), dim3(256), lds, st, (const float*)logits, ld, V, 2 * K, keys,
                            stats);
     else
-        hipLaunchKernelGGL(beam_chunk_kernel<bf16_t>, dim3(chunks, B * K), dim3(256), 0, st, (const bf16_t*)logits, ld, V, 2 * K,
+        hipLaunchKernelGGL(beam_chunk_kernel<bf16_t>, dim3(chunks, B * K), dim3(256), lds, st, (const bf16_t*)logits, ld, V, 2 * K,
                            keys, stats);
-    hipLaunchKernelGGL(beam_join_kernel, dim3(B), dim3(256), 0, st, keys, stats, scores, K, V, chunks, 2 * K, eos, out_scores,
+    hipLaunchKernelGGL(beam_join_kernel, dim3(B), dim3(JOIN_T), 0, st, keys, stats, scores, K, V, chunks, 2 * K, eos, out_scores,
                        out_tokens, out_parents, cand_scores, cand_tokens, cand_parents);
     return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
 }

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -40,8 +41,15 @@ class BeamStep(NamedTuple):
     cand_parents: torch.Tensor
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _address(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _gpu(name: str, *tensors: torch.Tensor) -> torch.device:
@@ -53,6 +61,11 @@ def _gpu(name: str, *tensors: torch.Tensor) -> torch.device:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError(f"{name} has no backward: call it under torch.no_grad() or detach its inputs")
     return tensors[0].device
+
+
+@functools.lru_cache(maxsize=64)
+def _select_workspace(B: int, K: int, V: int) -> int:
+    return _lib.load().asrk_beam_select_workspace_bytes(B, K, V)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, eos_token_id: Optional[int] = None) -> BeamStep:
@@ -89,14 +102,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, eos_token_id: Option
     scores = scores.contiguous()
     if ld < V:  # a single row, or rows that overlap
         logits, ld = logits.contiguous(), V
-    out = [torch.empty((B, n), dtype=t, device=dev) for n in (K, 2 * K) for t in (torch.float32, torch.int64, torch.int64)]
+    out = [scores.new_empty((B, n), dtype=t) for n in (K, 2 * K) for t in (torch.float32, torch.int64, torch.int64)]
     if B == 0:
         return BeamStep(*out)
     lib = _lib.load()
     with _on(dev):
-        ws = torch.empty((lib.asrk_beam_select_workspace_bytes(B, K, V),), dtype=torch.uint8, device=dev)
-        _lib.check(lib.asrk_beam_select(_lib.ptr(logits), _DT[logits.dtype], ld, _lib.ptr(scores), B, K, V, eos, *map(_lib.ptr, out),
-                                        _lib.ptr(ws), ws.numel(), _lib.current_stream()), "asrk_beam_select")
+        need = _select_workspace(B, K, V)
+        ws = scores.new_empty((need,), dtype=torch.uint8)
+        _lib.check(lib.asrk_beam_select(logits.data_ptr(), _DT[logits.dtype], ld, scores.data_ptr(), B, K, V, eos, *[t.data_ptr() for t in out],
+                                        ws.data_ptr(), need, _lib.stream_of(dev)), "asrk_beam_select")
     return BeamStep(*out)
 
 
@@ -121,8 +135,8 @@ def reorder_states(states: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
     if out.numel() == 0:
         return out
     with _on(dev):
-        _lib.check(_lib.load().asrk_reorder_rows(_lib.ptr(states), _lib.ptr(parents), B, K, states.numel() // (B * K) * states.element_size(),
-                                                 _lib.ptr(out), _lib.current_stream()), "asrk_reorder_rows")
+        _lib.check(_lib.load().asrk_reorder_rows(states.data_ptr(), parents.data_ptr(), B, K,
+                                                 states.numel() // (B * K) * states.element_size(), out.data_ptr(), _lib.stream_of(dev)), "asrk_reorder_rows")
     return out
 
 
@@ -211,7 +225,7 @@ class PagedKVCache:
         elif not 0 <= n <= self.max_len:
             raise ValueError(f"cannot add {n} tokens to sequences of at most {self.max_len}")
         with _on(self.device):
-            _lib.check(_lib.load().asrk_kv_extend(self._ref, _lib.ptr(each), n, _lib.current_stream()), "asrk_kv_extend")
+            _lib.check(_lib.load().asrk_kv_extend(self._ref, _address(each), n, _lib.stream_of(self.device)), "asrk_kv_extend")
 
     def reorder(self, parents: torch.Tensor) -> None:
         """Beam k of utterance b goes on as a copy of its beam ``parents[b, k]``; -1 empties it and gives its pages back.
@@ -221,14 +235,14 @@ class PagedKVCache:
             raise ValueError(f"parents must be [B, K] with B * K == {self.num_seqs} and K <= 32, got {list(parents.shape)}")
         self._mine("reorder", parents)
         with _on(self.device):
-            _lib.check(_lib.load().asrk_kv_reorder(self._ref, _lib.ptr(parents), parents.shape[1], _lib.current_stream()), "asrk_kv_reorder")
+            _lib.check(_lib.load().asrk_kv_reorder(self._ref, parents.data_ptr(), parents.shape[1], _lib.stream_of(self.device)), "asrk_kv_reorder")
 
     def compact(self) -> torch.Tensor:
         """Moves pages so that those in use are the first ones of the pool; returns their number (int32 [], on the device)."""
         if self._seq_stride != 1:
             raise ValueError("compact the cache itself, not a view of some of its sequences")
         with _on(self.device):
-            _lib.check(_lib.load().asrk_kv_compact(self._ref, _lib.current_stream()), "asrk_kv_compact")
+            _lib.check(_lib.load().asrk_kv_compact(self._ref, _lib.stream_of(self.device)), "asrk_kv_compact")
         return self.status[1]
 
     def check(self) -> None:
@@ -276,8 +290,8 @@ class PagedKVCache:
             k, v = k.contiguous(), v.contiguous()
             lds = tuple(k.stride()[:3])
         with _on(self.device):
-            _lib.check(_lib.load().asrk_kv_write(self._ref, layer, _lib.ptr(k), _lib.ptr(v), _DT[k.dtype], *lds, k.shape[1],
-                                                 _lib.current_stream()), "asrk_kv_write")
+            _lib.check(_lib.load().asrk_kv_write(self._ref, layer, k.data_ptr(), v.data_ptr(), _DT[k.dtype], *lds, k.shape[1],
+                                                 _lib.stream_of(self.device)), "asrk_kv_write")
 
     def read(self, first: Union[int, torch.Tensor], count: int, layer: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Tokens ``first`` .. ``first + count - 1`` of every sequence (an int, or an integer [num_seqs] tensor) as they are
@@ -301,8 +315,8 @@ class PagedKVCache:
         layer = 0 if layer is None else self._layer(layer)
         if count:
             with _on(self.device):
-                _lib.check(_lib.load().asrk_kv_read(self._ref, layer, layers, _lib.ptr(each), first, count, *map(_lib.ptr, out),
-                                                    _lib.current_stream()), "asrk_kv_read")
+                _lib.check(_lib.load().asrk_kv_read(self._ref, layer, layers, _address(each), first, count, out[0].data_ptr(), out[1].data_ptr(),
+                                                    _lib.stream_of(self.device)), "asrk_kv_read")
         return out[0], out[1]
 
     def attend(self, q: torch.Tensor, layer: int = 0, *, scale: Optional[float] = None, num_beams: int = 1) -> torch.Tensor:
@@ -320,7 +334,7 @@ class PagedKVCache:
             raise ValueError(f"{self.num_seqs} sequences are not groups of {num_beams} (at most 32)")
         self._mine("attend", q)
         layer = self._layer(layer)
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+        out = q.new_empty(q.shape)
         if out.numel() == 0:
             return out
         q, lds = self._rows(q)
@@ -328,8 +342,8 @@ class PagedKVCache:
         lib = _lib.load()
         with _on(self.device):
             need = lib.asrk_kv_attention_workspace_bytes(self._ref, n, heads, num_beams)
-            ws = torch.empty((need,), dtype=torch.uint8, device=self.device) if need else None
-            _lib.check(lib.asrk_kv_attention(self._ref, layer, _lib.ptr(q), *lds, n, heads, num_beams,
-                                             self.head_dim ** -0.5 if scale is None else float(scale), _lib.ptr(out), _lib.ptr(ws), need,
-                                             _lib.current_stream()), "asrk_kv_attention")
+            ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+            _lib.check(lib.asrk_kv_attention(self._ref, layer, q.data_ptr(), *lds, n, heads, num_beams,
+                                             self.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _address(ws), need,
+                                             _lib.stream_of(self.device)), "asrk_kv_attention")
         return out

@@ -322,7 +322,7 @@ class PagedKVCache:
     def attend(self, q: torch.Tensor, layer: int = 0, *, scale: Optional[float] = None, num_beams: int = 1) -> torch.Tensor:
         """Attention of the new tokens over one layer of the cache: bfloat16 [num_seqs, n, q_heads, head_dim] for ``q`` of that
         shape (any strides; query head j reads key/value head ``j // (q_heads // kv_heads)``).  Row i of sequence s sees the
-        tokens up to its own, ``starts[s] + i``; rows behind ``lens[s]`` are zero.  ``scale`` is ``head_dim ** -0.5`` by default.
+        tokens up to its own, ``starts[s] + i``; rows behind ``lens[s]`` are zero.  ``scale`` (positive) is ``head_dim ** -0.5`` by default.
 
         ``num_beams`` consecutive sequences are worked on together, and pages that they share are read once.  It changes
         nothing else: the beams may share any pages, or none."""
@@ -332,6 +332,9 @@ class PagedKVCache:
             raise ValueError("q must be bfloat16")
         if not 1 <= num_beams <= 32 or self.num_seqs % num_beams:
             raise ValueError(f"{self.num_seqs} sequences are not groups of {num_beams} (at most 32)")
+        scale = self.head_dim ** -0.5 if scale is None else float(scale)
+        if not 0 < scale < float("inf"):
+            raise ValueError(f"scale must be positive and finite, got {scale}")
         self._mine("attend", q)
         layer = self._layer(layer)
         out = q.new_empty(q.shape)
@@ -344,6 +347,6 @@ class PagedKVCache:
             need = lib.asrk_kv_attention_workspace_bytes(self._ref, n, heads, num_beams)
             ws = q.new_empty((need,), dtype=torch.uint8) if need else None
             _lib.check(lib.asrk_kv_attention(self._ref, layer, q.data_ptr(), *lds, n, heads, num_beams,
-                                             self.head_dim ** -0.5 if scale is None else float(scale), out.data_ptr(), _address(ws), need,
+                                             scale, out.data_ptr(), _address(ws), need,
                                              _lib.stream_of(self.device)), "asrk_kv_attention")
         return out

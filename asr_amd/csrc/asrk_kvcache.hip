@@ -68,9 +68,17 @@ __device__ int list_pages(const int* refs, int from, int to, int want, int* out,
     for (int base = from; base < to && found < want; base += MANAGE_T * PER) {
         const int at = base + threadIdx.x * PER;
         uint32_t mine = 0;
+        if (at + PER <= to && !(((uintptr_t)(refs + at)) & 15)) {
+            u32x4 r[PER / 4];
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            if (at + i < to) mine |= (FREE == (refs[at + i] == 0) ? 1u : 0u) << i;
+            for (int i = 0; i < PER / 4; ++i) r[i] = reinterpret_cast<const u32x4*>(refs + at)[i];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) mine |= (FREE == (r[i / 4][i % 4] == 0) ? 1u : 0u) << i;
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (at + i < to) mine |= (FREE == (refs[at + i] == 0) ? 1u : 0u) << i;
+        }
         int total;
         int r = found + block_scan_exclusive(__popc(mine), lds, total);
         while (mine) {
@@ -108,8 +116,7 @@ __global__ __launch_bounds__(MANAGE_T) void kv_extend_kernel(asrk_kv_cache c, co
             }
         }
     }
-    __threadfence();
-    __syncthreads();
+    __syncthreads();  // one workgroup: its atomics are done (at L2) and are read there, past L1
     const bool fits = flags == 0;
     __syncthreads();
     int need_all = 0;
@@ -139,7 +146,6 @@ __global__ __launch_bounds__(MANAGE_T) void kv_extend_kernel(asrk_kv_cache c, co
     if (fits && need_all > 0) {
         got = need_all <= c.num_pages ? list_pages<true>(c.refs, 0, c.num_pages, need_all, sc.list, lds) : 0;
         if (got < need_all && threadIdx.x == 0) flags = ASRK_KV_OUT_OF_PAGES;
-        __threadfence();
         __syncthreads();
     }
     const bool go = fits && got == need_all;
@@ -259,7 +265,6 @@ __global__ __launch_bounds__(MANAGE_T) void kv_compact_plan_kernel(asrk_kv_cache
     int* high = sc.lowest;
     const int n = list_pages<true>(c.refs, 0, used, used, holes, lds);
     list_pages<false>(c.refs, used, P, n, high, lds);
-    __threadfence();
     __syncthreads();
     for (int r = threadIdx.x; r < n; r += MANAGE_T) {
         const int src = load_agent(&high[r]), dst = load_agent(&holes[r]);
@@ -294,19 +299,19 @@ __global__ __launch_bounds__(256) void kv_rename_kernel(asrk_kv_cache c) {
 // ---- tokens in
 
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float* x);
+struct Eight;  // eight values as they are loaded
 template <>
-__device__ __forceinline__ void load8<float>(const float* p, float* x) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
-}
+struct Eight<float> {
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = reinterpret_cast<const f32x4*>(p)[0]; b = reinterpret_cast<const f32x4*>(p)[1]; }
+    __device__ __forceinline__ float operator[](int i) const { return i < 4 ? a[i] : b[i - 4]; }
+};
 template <>
-__device__ __forceinline__ void load8<bf16_t>(const bf16_t* p, float* x) {
-    const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
-}
+struct Eight<bf16_t> {
+    bf16x8 a;
+    __device__ __forceinline__ void load(const bf16_t* p) { a = *reinterpret_cast<const bf16x8*>(p); }
+    __device__ __forceinline__ float operator[](int i) const { return (float)a[i]; }
+};
 
 __device__ __forceinline__ int exponent_of(float most) {  // smallest e with most <= 448 2^e, clamped
     const uint32_t b = __float_as_uint(most);
@@ -316,7 +321,8 @@ __device__ __forceinline__ int exponent_of(float most) {  // smallest e with mos
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // normal range only
 
 // four values / scale -> four e4m3 bytes, to the nearest, ties to even; not finite: NaN
-__device__ __forceinline__ uint32_t to_e4m3x4(const float* x, float inv) {
+__device__ __forceinline__ uint32_t to_e4m3x4(float x0, float x1, float x2, float x3, float inv) {
+    const float x[4] = {x0, x1, x2, x3};
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i] * inv, -448.f, 448.f);
@@ -330,27 +336,29 @@ __device__ __forceinline__ uint32_t to_e4m3x4(const float* x, float inv) {
 }
 // four e4m3 bytes times 2^shift (shift <= 0), rounded again
 __device__ __forceinline__ uint32_t shift_e4m3x4(uint32_t u, float factor) {
-    float x[4];
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false);
     const auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, true);
-    x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
-    return to_e4m3x4(x, factor);
+    return to_e4m3x4(a[0], a[1], b[0], b[1], factor);
 }
 
-// One workgroup per (page that new tokens touch, head, sequence).  Two passes over the new rows (the second from cache):
-// the largest magnitude, then the bytes.  Older tokens of the page are only touched if the exponent grows.
-template <class T>
-__global__ __launch_bounds__(256) void kv_write_kernel(asrk_kv_cache c, const T* __restrict__ k, const T* __restrict__ v, int64_t seq_ld, int64_t row_ld,
-                                int64_t head_ld, int n, int64_t layer) {
+// One workgroup per (head, page that new tokens touch, sequence).  The new rows are read once, into registers: the largest
+// magnitude first, then the bytes.  Value bytes are turned through LDS four by four (rows of D + 4 bytes: 16 x 4 lanes read
+// different banks).  Older tokens of the page are only touched if the exponent grows.  Heads vary fastest over the grid:
+// neighbours read, and the rows are whole, together.
+template <class T, int D, int THREADS, int U>  // U pieces of eight values per thread and tensor
+__global__ __launch_bounds__(THREADS) void kv_write_kernel(asrk_kv_cache c, const T* __restrict__ k, const T* __restrict__ v, int64_t seq_ld,
+                                                           int64_t row_ld, int64_t head_ld, int n, int64_t layer) {
+    constexpr int PER = D / 8, LINE = D + 4;
+    __shared__ __attribute__((aligned(16))) uint8_t turn[ASRK_KV_PAGE * LINE];
     __shared__ uint32_t most[2];
     __shared__ int odd;
-    const int D = c.head_dim, H = c.kv_heads, M = c.max_pages;
-    const int s = blockIdx.z, h = blockIdx.y;
+    const int H = c.kv_heads, M = c.max_pages;
+    const int s = blockIdx.z, h = blockIdx.x;
     const int64_t slot = (int64_t)s * c.seq_stride;
     const int start = c.starts[slot];
     int rows = c.lens[slot] - start;
     rows = rows < n ? rows : n;
-    const int pj = start / ASRK_KV_PAGE + blockIdx.x;
+    const int pj = start / ASRK_KV_PAGE + blockIdx.y;
     const int lo = start > pj * ASRK_KV_PAGE ? start : pj * ASRK_KV_PAGE;
     const int hi = start + rows < (pj + 1) * ASRK_KV_PAGE ? start + rows : (pj + 1) * ASRK_KV_PAGE;
     if (lo >= hi || pj >= M) return;
@@ -362,26 +370,34 @@ __global__ __launch_bounds__(256) void kv_write_kernel(asrk_kv_cache c, const T*
     uint8_t* vp = kp + ASRK_KV_PAGE * D;
     int8_t* ep = c.exps + at * 4;
     const int64_t base = (int64_t)s * seq_ld + (int64_t)h * head_ld - (int64_t)(start - pj * ASRK_KV_PAGE) * row_ld;  // row of token t: base + t * row_ld
+    const int units = (t1 - t0) * PER;
+    Eight<T> kx[U], vx[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int u = j * THREADS + threadIdx.x;
+        if (u < units) {
+            const int64_t o = base + (int64_t)(t0 + u / PER) * row_ld + u % PER * 8;
+            kx[j].load(k + o);
+            vx[j].load(v + o);
+        }
+    }
     const int old = *reinterpret_cast<const int*>(ep);
     if (threadIdx.x < 2) most[threadIdx.x] = 0;
     if (threadIdx.x == 0) odd = 0;
     __syncthreads();
-    const int per = D / 8, units = (t1 - t0) * per;
     float mk = 0.f, mv = 0.f;
     bool nan_v = false;
-    for (int u = threadIdx.x; u < units; u += blockDim.x) {
-        const int64_t o = base + (int64_t)(t0 + u / per) * row_ld + (u % per) * 8;
-        float x[8], y[8];
-        load8(k + o, x);
-        load8(v + o, y);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float a = fabsf(x[i]), b = fabsf(y[i]);
-            mk = a < __builtin_inff() ? fmaxf(mk, a) : mk;
-            mv = b < __builtin_inff() ? fmaxf(mv, b) : mv;
-            nan_v |= !(b < __builtin_inff());
+    for (int j = 0; j < U; ++j)
+        if (j * THREADS + threadIdx.x < units) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = fabsf(kx[j][i]), y = fabsf(vx[j][i]);
+                mk = x < __builtin_inff() ? fmaxf(mk, x) : mk;
+                mv = y < __builtin_inff() ? fmaxf(mv, y) : mv;
+                nan_v |= !(y < __builtin_inff());
+            }
         }
-    }
     mk = wave_max(mk);
     mv = wave_max(mv);
     nan_v = __any(nan_v);
@@ -402,43 +418,65 @@ __global__ __launch_bounds__(256) void kv_write_kernel(asrk_kv_cache c, const T*
     }
     const float ik = pow2(-ek), iv = pow2(-ev);
     if (t0 > 0 && fk != 1.f)
-        for (int u = threadIdx.x; u < t0 * D / 4; u += blockDim.x) ((uint32_t*)kp)[u] = shift_e4m3x4(((const uint32_t*)kp)[u], fk);
-    for (int u = threadIdx.x; u < units; u += blockDim.x) {
-        const int t = t0 + u / per, d = (u % per) * 8;
-        float x[8];
-        load8(k + base + (int64_t)t * row_ld + d, x);
-        u32x2 w;
-        w[0] = to_e4m3x4(x, ik);
-        w[1] = to_e4m3x4(x + 4, ik);
-        *reinterpret_cast<u32x2*>(kp + t * D + d) = w;
+        for (int u = threadIdx.x; u < t0 * D / 4; u += THREADS) ((uint32_t*)kp)[u] = shift_e4m3x4(((const uint32_t*)kp)[u], fk);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        const int u = j * THREADS + threadIdx.x;
+        if (u < units) {
+            const int t = t0 + u / PER, d = u % PER * 8;
+            u32x2 w;
+            w[0] = to_e4m3x4(kx[j][0], kx[j][1], kx[j][2], kx[j][3], ik);
+            w[1] = to_e4m3x4(kx[j][4], kx[j][5], kx[j][6], kx[j][7], ik);
+            *reinterpret_cast<u32x2*>(kp + t * D + d) = w;
+            uint32_t* line = reinterpret_cast<uint32_t*>(turn + t * LINE + d);
+            line[0] = to_e4m3x4(vx[j][0], vx[j][1], vx[j][2], vx[j][3], iv);
+            line[1] = to_e4m3x4(vx[j][4], vx[j][5], vx[j][6], vx[j][7], iv);
+        }
     }
-    // values: four tokens of one d at a time; lanes run over d, so that the rows are read in whole lines
+    __syncthreads();
+    // four tokens by four d's per step; lanes run over the tokens first, so that stores are whole lines
     const bool shift = t0 > 0 && fv != 1.f;
-    const int g0 = shift ? 0 : t0 / 4, g1 = (t1 + 3) / 4;
-    for (int u = threadIdx.x; u < (g1 - g0) * D; u += blockDim.x) {
-        const int d = u % D, g = g0 + u / D;
-        uint32_t* p = (uint32_t*)(vp + d * ASRK_KV_PAGE + g * 4);
-        float x[4];
-        uint32_t mask = 0;
+    const int g0 = shift ? 0 : t0 / 4, gs = (t1 + 3) / 4 - g0;
+    for (int u = threadIdx.x; u < gs * (D / 4); u += THREADS) {
+        const int g = g0 + u % gs, d = u / gs * 4;
+        uint32_t w[4], x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint32_t*>(turn + (g * 4 + i) * LINE + d);  // token 4 g + i: d .. d + 3
+        const uint32_t a0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), a1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
+        const uint32_t b0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400), b1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+        x[0] = __builtin_amdgcn_perm(b0, a0, 0x05040100);  // d: tokens 4 g .. 4 g + 3
+        x[1] = __builtin_amdgcn_perm(b0, a0, 0x07060302);
+        x[2] = __builtin_amdgcn_perm(b1, a1, 0x05040100);
+        x[3] = __builtin_amdgcn_perm(b1, a1, 0x07060302);
+        uint32_t mask = 0;  // of the new tokens among the four
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mask |= g * 4 + i >= t0 && g * 4 + i < t1 ? 0xffu << (8 * i) : 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int t = g * 4 + i;
-            const bool in = t >= t0 && t < t1;
-            x[i] = in ? (float)v[base + (int64_t)t * row_ld + d] : 0.f;
-            mask |= in ? 0xffu << (8 * i) : 0;
+            uint32_t* p = reinterpret_cast<uint32_t*>(vp + (d + i) * ASRK_KV_PAGE + g * 4);
+            if (mask != 0xffffffffu) {
+                uint32_t o = *p;
+                if (shift) o = shift_e4m3x4(o, fv);
+                x[i] = (x[i] & mask) | (o & ~mask);
+            }
+            *p = x[i];
         }
-        uint32_t w = to_e4m3x4(x, iv);
-        if (mask != 0xffffffffu) {
-            uint32_t o = *p;
-            if (shift) o = shift_e4m3x4(o, fv);
-            w = (w & mask) | (o & ~mask);
-        }
-        *p = w;
     }
     if (threadIdx.x == 0) {
         const int flag = odd | (t0 > 0 ? (old >> 16) & 1 : 0);
         *reinterpret_cast<int*>(ep) = (ek & 0xff) | ((ev & 0xff) << 8) | (flag << 16);
     }
+}
+template <class T, int D>
+void launch_write(const asrk_kv_cache* c, const void* k, const void* v, int64_t seq_ld, int64_t row_ld, int64_t head_ld, int n, int layer,
+                  hipStream_t st) {
+    const dim3 grid(c->kv_heads, (unsigned)(((int64_t)n + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1), c->num_seqs);
+    if (n == 1)  // D / 8 pieces of work: one wave
+        hipLaunchKernelGGL((kv_write_kernel<T, D, 64, 1>), grid, dim3(64), 0, st, *c, (const T*)k, (const T*)v, seq_ld, row_ld, head_ld, n,
+                           (int64_t)layer);
+    else
+        hipLaunchKernelGGL((kv_write_kernel<T, D, 256, D / 32>), grid, dim3(256), 0, st, *c, (const T*)k, (const T*)v, seq_ld, row_ld,
+                           head_ld, n, (int64_t)layer);
 }
 
 // ---- tokens out
@@ -449,11 +487,11 @@ __global__ __launch_bounds__(256) void kv_read_kernel(asrk_kv_cache c, const int
                                                       int layer0, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out) {
     __shared__ uint32_t turn[128 * 17];
     const int D = c.head_dim, H = c.kv_heads, M = c.max_pages;
-    const int h = blockIdx.y;
+    const int h = blockIdx.x;
     const int s = blockIdx.z % c.num_seqs, l = blockIdx.z / c.num_seqs;
     const int64_t slot = (int64_t)s * c.seq_stride;
     const int64_t first = first_each ? first_each[s] : first_all;
-    const int64_t pj = (first < 0 ? -((-first + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE) : first / ASRK_KV_PAGE) + blockIdx.x;
+    const int64_t pj = (first < 0 ? -((-first + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE) : first / ASRK_KV_PAGE) + blockIdx.y;
     const int64_t t_lo = first - pj * ASRK_KV_PAGE, t_hi = first + count - pj * ASRK_KV_PAGE;  // asked tokens within the page
     if (t_hi <= 0) return;
     const int lo = t_lo > 0 ? (int)t_lo : 0, hi = t_hi < ASRK_KV_PAGE ? (int)t_hi : ASRK_KV_PAGE;
@@ -526,7 +564,8 @@ int asrk_kv_check(const asrk_kv_cache* c) {
         return ASRK_ERR_SHAPE;
     if (c->head_dim != 64 && c->head_dim != 128) return ASRK_ERR_SHAPE;
     if (c->num_layers > 65535 || c->kv_heads > 65535 || c->num_seqs > 65535 || (int64_t)c->num_seqs * c->seq_stride > 0x7fffffff ||
-        c->max_pages > 0x7fffffff / ASRK_KV_PAGE || c->num_pages > 0x3fffffff)
+        (int64_t)c->num_seqs * c->seq_stride * c->max_pages > 0x7fffffff || c->max_pages > 0x7fffffff / ASRK_KV_PAGE ||
+        c->num_pages > 0x3fffffff)
         return ASRK_ERR_SHAPE;
     if (((uintptr_t)c->kv & 15) || ((uintptr_t)c->exps & 15) || ((uintptr_t)c->table & 3) || ((uintptr_t)c->lens & 3) ||
         ((uintptr_t)c->starts & 3) || ((uintptr_t)c->refs & 15) || ((uintptr_t)c->status & 3) || ((uintptr_t)c->scratch & 15))
@@ -582,15 +621,12 @@ extern "C" int asrk_kv_write(const asrk_kv_cache* c, int layer, const void* k, c
     if (layer < 0 || layer >= c->num_layers || n <= 0 || seq_ld < 0 || row_ld < 0 || head_ld < 0) return ASRK_ERR_SHAPE;
     const int per = dtype == ASRK_F32 ? 4 : 8;  // values in 16 bytes
     if (((uintptr_t)k & 15) || ((uintptr_t)v & 15) || seq_ld % per || row_ld % per || head_ld % per) return ASRK_ERR_ALIGN;
-    const dim3 grid((unsigned)(((int64_t)n + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1), c->kv_heads, c->num_seqs);
-    const dim3 block(n == 1 ? 64 : 256);  // a single token has D / 8 pieces of work per tensor
+    if (((int64_t)n + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1 > 65535) return ASRK_ERR_SHAPE;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == ASRK_F32)
-        hipLaunchKernelGGL(kv_write_kernel<float>, grid, block, 0, st, *c, (const float*)k, (const float*)v, seq_ld, row_ld, head_ld, n,
-                           (int64_t)layer);
-    else
-        hipLaunchKernelGGL(kv_write_kernel<bf16_t>, grid, block, 0, st, *c, (const bf16_t*)k, (const bf16_t*)v, seq_ld, row_ld, head_ld,
-                           n, (int64_t)layer);
+    if (dtype == ASRK_F32 && c->head_dim == 64) launch_write<float, 64>(c, k, v, seq_ld, row_ld, head_ld, n, layer, st);
+    else if (dtype == ASRK_F32) launch_write<float, 128>(c, k, v, seq_ld, row_ld, head_ld, n, layer, st);
+    else if (c->head_dim == 64) launch_write<bf16_t, 64>(c, k, v, seq_ld, row_ld, head_ld, n, layer, st);
+    else launch_write<bf16_t, 128>(c, k, v, seq_ld, row_ld, head_ld, n, layer, st);
     return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
 }
 
@@ -601,7 +637,9 @@ extern "C" int asrk_kv_read(const asrk_kv_cache* c, int layer, int layers, const
     if (layer < 0 || layers <= 0 || layer + (int64_t)layers > c->num_layers || count <= 0) return ASRK_ERR_SHAPE;
     if (((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15)) return ASRK_ERR_ALIGN;
     if ((int64_t)layers * c->num_seqs > 65535) return ASRK_ERR_SHAPE;
-    const dim3 grid((unsigned)(((int64_t)count + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1), c->kv_heads, c->num_seqs * layers);
+    const int64_t parts = ((int64_t)count + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1;  // pages that `count` tokens can touch
+    if (parts > 65535) return ASRK_ERR_SHAPE;
+    const dim3 grid(c->kv_heads, (unsigned)parts, c->num_seqs * layers);
     hipLaunchKernelGGL(kv_read_kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, first_each, first_all, count, layer, (bf16_t*)k_out,
                        (bf16_t*)v_out);
     return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;

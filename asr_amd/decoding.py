@@ -173,7 +173,7 @@ class PagedKVCache:
             raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
         max_pages = -(-max_len // PAGE)
         num_pages = num_seqs * max_pages if num_pages is None else num_pages
-        if num_pages < 1 or num_pages > 0x3FFFFFFF or max_pages > 0x7FFFFFFF // PAGE:
+        if num_pages < 1 or num_pages > 0x3FFFFFFF or max_pages > 0x7FFFFFFF // PAGE or num_seqs * max_pages > 0x7FFFFFFF:
             raise ValueError(f"num_pages {num_pages} / max_len {max_len} out of range")
         device = torch.device(device)
         if device.type != "cuda":
@@ -285,6 +285,8 @@ class PagedKVCache:
         layer = self._layer(layer)
         if k.shape[1] == 0:
             return
+        if k.shape[1] > 65534 * PAGE:
+            raise ValueError(f"cannot write {k.shape[1]} tokens in one call")
         (k, lds), (v, v_lds) = self._rows(k), self._rows(v)
         if lds != v_lds:
             k, v = k.contiguous(), v.contiguous()
@@ -305,8 +307,8 @@ class PagedKVCache:
             each, first = first.to(torch.int32).contiguous(), 0
         elif not 0 <= first <= self.max_len:
             raise ValueError(f"first {first} of sequences of at most {self.max_len}")
-        if not 0 <= count <= 0x7FFFFFFF:
-            raise ValueError(f"cannot read {count} tokens")
+        if not 0 <= count <= 65534 * PAGE:
+            raise ValueError(f"cannot read {count} tokens in one call")
         layers = self.num_layers if layer is None else 1
         if layers * self.num_seqs > 65535:
             raise ValueError("read one layer at a time: layers * num_seqs passes 65535")

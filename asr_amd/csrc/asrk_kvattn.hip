@@ -275,7 +275,7 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
                 const float now = groups_max(top) * a.c;  // c > 0
                 if (__any(now > m[x] + 8.f) || up != unit) {
                     KEEP_BRANCH();
-                    const float to = fmaxf(m[x], now);
+                    const float to = now > m[x] + 8.f ? now : m[x];  // by the column alone: its bits do not depend on its neighbours
                     const float back = to > NEG_INF ? __builtin_amdgcn_exp2f(m[x] - to) : 0.f;
                     m[x] = to;
 #pragma unroll

@@ -16,7 +16,6 @@ libasrk.so; there is no CPU path.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import NamedTuple, Optional, Tuple, Union
@@ -41,11 +40,17 @@ class BeamStep(NamedTuple):
     cand_parents: torch.Tensor
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(device: torch.device):
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _call(name: str, device: torch.device, *args) -> None:
+    """One entry point of libasrk.so on the current stream of ``device`` (a step makes hundreds of calls: no context manager
+    and no Stream object where the device is current anyway)."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _lib.stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _lib.stream_of(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _address(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -53,14 +58,15 @@ def _address(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _gpu(name: str, *tensors: torch.Tensor) -> torch.device:
+    dev = tensors[0].device
     for t in tensors:
         if not t.is_cuda:
             raise _lib.AsrkError(f"{name} runs on a ROCm GPU only (there is no CPU fallback)")
-        if t.device != tensors[0].device:
-            raise ValueError(f"{name}: tensors on {tensors[0].device} and {t.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no backward: call it under torch.no_grad() or detach its inputs")
-    return tensors[0].device
+        if t.device != dev:
+            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} has no backward: call it under torch.no_grad() or detach its inputs")
+    return dev
 
 
 @functools.lru_cache(maxsize=64)
@@ -102,22 +108,20 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, eos_token_id: Option
     scores = scores.contiguous()
     if ld < V:  # a single row, or rows that overlap
         logits, ld = logits.contiguous(), V
-    out = [scores.new_empty((B, n), dtype=t) for n in (K, 2 * K) for t in (torch.float32, torch.int64, torch.int64)]
-    if B == 0:
-        return BeamStep(*out)
-    lib = _lib.load()
-    with _on(dev):
+    out = (scores.new_empty((B, K)), *scores.new_empty((2, B, K), dtype=torch.int64).unbind(0),
+           scores.new_empty((B, 2 * K)), *scores.new_empty((2, B, 2 * K), dtype=torch.int64).unbind(0))
+    if B:
         need = _select_workspace(B, K, V)
         ws = scores.new_empty((need,), dtype=torch.uint8)
-        _lib.check(lib.asrk_beam_select(logits.data_ptr(), _DT[logits.dtype], ld, scores.data_ptr(), B, K, V, eos, *[t.data_ptr() for t in out],
-                                        ws.data_ptr(), need, _lib.stream_of(dev)), "asrk_beam_select")
+        _call("asrk_beam_select", dev, logits.data_ptr(), _DT[logits.dtype], ld, scores.data_ptr(), B, K, V, eos, *[t.data_ptr() for t in out],
+              ws.data_ptr(), need)
     return BeamStep(*out)
 
 
 def _check_parents(name: str, parents: torch.Tensor) -> torch.Tensor:
     if parents.dim() != 2 or parents.dtype != torch.int64:
         raise ValueError(f"{name}: parents must be an int64 [B, K] tensor")
-    return parents.contiguous()
+    return parents if parents.is_contiguous() else parents.contiguous()
 
 
 def reorder_states(states: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
@@ -132,11 +136,9 @@ def reorder_states(states: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
     dev = _gpu("reorder_states", states, parents)
     states = states.contiguous()
     out = torch.empty_like(states)
-    if out.numel() == 0:
-        return out
-    with _on(dev):
-        _lib.check(_lib.load().asrk_reorder_rows(states.data_ptr(), parents.data_ptr(), B, K,
-                                                 states.numel() // (B * K) * states.element_size(), out.data_ptr(), _lib.stream_of(dev)), "asrk_reorder_rows")
+    if out.numel():
+        _call("asrk_reorder_rows", dev, states.data_ptr(), parents.data_ptr(), B, K, states.numel() // (B * K) * states.element_size(),
+              out.data_ptr())
     return out
 
 
@@ -221,11 +223,10 @@ class PagedKVCache:
             if n.dim() != 1 or n.shape[0] != self.num_seqs or n.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"n must be an int or an integer [{self.num_seqs}] tensor")
             self._mine("extend", n)
-            each, n = n.to(torch.int32).contiguous(), 0
+            each, n = self._int32(n), 0
         elif not 0 <= n <= self.max_len:
             raise ValueError(f"cannot add {n} tokens to sequences of at most {self.max_len}")
-        with _on(self.device):
-            _lib.check(_lib.load().asrk_kv_extend(self._ref, _address(each), n, _lib.stream_of(self.device)), "asrk_kv_extend")
+        _call("asrk_kv_extend", self.device, self._ref, _address(each), n)
 
     def reorder(self, parents: torch.Tensor) -> None:
         """Beam k of utterance b goes on as a copy of its beam ``parents[b, k]``; -1 empties it and gives its pages back.
@@ -234,15 +235,13 @@ class PagedKVCache:
         if parents.numel() != self.num_seqs or parents.shape[1] > 32:
             raise ValueError(f"parents must be [B, K] with B * K == {self.num_seqs} and K <= 32, got {list(parents.shape)}")
         self._mine("reorder", parents)
-        with _on(self.device):
-            _lib.check(_lib.load().asrk_kv_reorder(self._ref, parents.data_ptr(), parents.shape[1], _lib.stream_of(self.device)), "asrk_kv_reorder")
+        _call("asrk_kv_reorder", self.device, self._ref, parents.data_ptr(), parents.shape[1])
 
     def compact(self) -> torch.Tensor:
         """Moves pages so that those in use are the first ones of the pool; returns their number (int32 [], on the device)."""
         if self._seq_stride != 1:
             raise ValueError("compact the cache itself, not a view of some of its sequences")
-        with _on(self.device):
-            _lib.check(_lib.load().asrk_kv_compact(self._ref, _lib.stream_of(self.device)), "asrk_kv_compact")
+        _call("asrk_kv_compact", self.device, self._ref)
         return self.status[1]
 
     def check(self) -> None:
@@ -255,8 +254,14 @@ class PagedKVCache:
     # ---- tokens
 
     def _mine(self, name: str, *tensors: torch.Tensor) -> None:
-        if _gpu(f"PagedKVCache.{name}", *tensors) != self.device:
+        if _gpu(name, *tensors) != self.device:
             raise ValueError(f"{name}: the cache is on {self.device}, the tensors are on {tensors[0].device}")
+
+    @staticmethod
+    def _int32(x: torch.Tensor) -> torch.Tensor:
+        if x.dtype == torch.int64:
+            x = x.clamp(-0x80000000, 0x7FFFFFFF).to(torch.int32)  # what does not fit stays out of range
+        return x.contiguous()
 
     def _layer(self, layer: int) -> int:
         if not 0 <= layer < self.num_layers:
@@ -291,9 +296,7 @@ class PagedKVCache:
         if lds != v_lds:
             k, v = k.contiguous(), v.contiguous()
             lds = tuple(k.stride()[:3])
-        with _on(self.device):
-            _lib.check(_lib.load().asrk_kv_write(self._ref, layer, k.data_ptr(), v.data_ptr(), _DT[k.dtype], *lds, k.shape[1],
-                                                 _lib.stream_of(self.device)), "asrk_kv_write")
+        _call("asrk_kv_write", self.device, self._ref, layer, k.data_ptr(), v.data_ptr(), _DT[k.dtype], *lds, k.shape[1])
 
     def read(self, first: Union[int, torch.Tensor], count: int, layer: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Tokens ``first`` .. ``first + count - 1`` of every sequence (an int, or an integer [num_seqs] tensor) as they are
@@ -304,7 +307,7 @@ class PagedKVCache:
             if first.dim() != 1 or first.shape[0] != self.num_seqs or first.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"first must be an int or an integer [{self.num_seqs}] tensor")
             self._mine("read", first)
-            each, first = first.to(torch.int32).contiguous(), 0
+            each, first = self._int32(first), 0
         elif not 0 <= first <= self.max_len:
             raise ValueError(f"first {first} of sequences of at most {self.max_len}")
         if not 0 <= count <= 65534 * PAGE:
@@ -316,9 +319,7 @@ class PagedKVCache:
         out = [torch.empty(shape if layer is not None else (layers, *shape), dtype=torch.bfloat16, device=self.device) for _ in range(2)]
         layer = 0 if layer is None else self._layer(layer)
         if count:
-            with _on(self.device):
-                _lib.check(_lib.load().asrk_kv_read(self._ref, layer, layers, _address(each), first, count, out[0].data_ptr(), out[1].data_ptr(),
-                                                    _lib.stream_of(self.device)), "asrk_kv_read")
+            _call("asrk_kv_read", self.device, self._ref, layer, layers, _address(each), first, count, out[0].data_ptr(), out[1].data_ptr())
         return out[0], out[1]
 
     def attend(self, q: torch.Tensor, layer: int = 0, *, scale: Optional[float] = None, num_beams: int = 1) -> torch.Tensor:
@@ -327,7 +328,7 @@ class PagedKVCache:
         tokens up to its own, ``starts[s] + i``; rows behind ``lens[s]`` are zero.  ``scale`` (positive) is ``head_dim ** -0.5`` by default.
 
         ``num_beams`` consecutive sequences are worked on together, and pages that they share are read once.  It changes
-        nothing else: the beams may share any pages, or none."""
+        no result but for rounding: the beams may share any pages, or none."""
         if q.dim() != 4 or q.shape[0] != self.num_seqs or q.shape[3] != self.head_dim or q.shape[2] < 1 or q.shape[2] % self.kv_heads:
             raise ValueError(f"q must be [{self.num_seqs}, n, a multiple of {self.kv_heads}, {self.head_dim}], got {list(q.shape)}")
         if q.dtype != torch.bfloat16:
@@ -344,11 +345,7 @@ class PagedKVCache:
             return out
         q, lds = self._rows(q)
         n, heads = q.shape[1], q.shape[2]
-        lib = _lib.load()
-        with _on(self.device):
-            need = lib.asrk_kv_attention_workspace_bytes(self._ref, n, heads, num_beams)
-            ws = q.new_empty((need,), dtype=torch.uint8) if need else None
-            _lib.check(lib.asrk_kv_attention(self._ref, layer, q.data_ptr(), *lds, n, heads, num_beams,
-                                             scale, out.data_ptr(), _address(ws), need,
-                                             _lib.stream_of(self.device)), "asrk_kv_attention")
+        need = _lib.load().asrk_kv_attention_workspace_bytes(self._ref, n, heads, num_beams)
+        ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+        _call("asrk_kv_attention", self.device, self._ref, layer, q.data_ptr(), *lds, n, heads, num_beams, scale, out.data_ptr(), _address(ws), need)
         return out

@@ -1,4 +1,5 @@
-"""Greedy-decode evaluation harness: the reference's ``evaluate_samples``
+"""Decode and evaluation harness: ``beam_generate``, beam search for a decoder over the paged 8-bit cache of
+``asr_amd.decoding``, and the greedy-decode evaluation: the reference's ``evaluate_samples``
 (src/train.py:36-82) and the prompt assembly of ``ASRModel.generate`` (src/modeling.py:296-334) on top of this
 package's extractor / encoder / projector / splice, plus a word error rate that needs no ``evaluate`` / ``jiwer``.
 
@@ -10,7 +11,7 @@ installed in this environment, so agreement with it is by definition and known-a
 """
 from __future__ import annotations
 
-from typing import Iterable, List, Sequence, Tuple
+from typing import Iterable, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -58,6 +59,79 @@ def build_generate_embeds(prompt_embeds: torch.Tensor, prompt_ids: torch.Tensor,
     except ValueError as e:
         raise ValueError("'<|audio_chunk|>' token not found in instruction.") from e  # :314-315
     return first.expand(audio_embeds.shape[0], -1, -1) if audio_embeds.shape[0] > 1 else first
+
+
+@torch.no_grad()
+def beam_generate(decoder, inputs_embeds: torch.Tensor, *, num_beams: int = 5, max_new_tokens: int = 100,
+                  eos_token_id: Optional[int] = None, length_penalty: float = 1.0, prompt_lens: Optional[torch.Tensor] = None,
+                  check_every: int = 8) -> Tuple[List[List[int]], torch.Tensor]:
+    """Beam search from prompt embeddings, as ``decoder.generate(inputs_embeds=..., num_beams=...)`` of the reference's last
+    lines (src/modeling.py:329-334) does it, on the device: the selection, the paged 8-bit cache and its attention are those
+    of ``asr_amd.decoding``, and the host is asked only every ``check_every`` steps whether all utterances are done.
+
+    ``inputs_embeds`` [B, P, D] on the GPU (``build_generate_embeds``, ``splice_audio_embeddings``), ``prompt_lens`` int [B] if
+    the prompts are right-padded.  ``decoder`` has ``num_layers``, ``kv_heads`` and ``head_dim``, ``embed(tokens [S]) -> [S, D]``,
+    and is called as ``decoder(embeds [S, n, D], cache, num_beams) -> logits [S, V]`` of every sequence's last new token; for
+    each layer it does ``cache.write(k, v, layer=l)`` and ``cache.attend(q, layer=l, num_beams=num_beams)``, and finds the new
+    tokens' positions from ``cache.starts`` on.
+
+    A hypothesis ends with ``eos_token_id`` (which is not returned) when it is among the best ``num_beams`` continuations of
+    its utterance; its score is its log-probability over its length (the end counted) to the power ``length_penalty``.  An
+    utterance is done when it has ``num_beams`` of them and its best running beam, at its present length, is no better than
+    the worst.  Returns the best hypothesis of every utterance and the scores, float32 [B]."""
+    from .decoding import PAGE, PagedKVCache, beam_select, reorder_states
+
+    if inputs_embeds.dim() != 3 or inputs_embeds.shape[0] < 1 or inputs_embeds.shape[1] < 1:
+        raise ValueError("inputs_embeds must be [B, P, D]")
+    if max_new_tokens < 1 or check_every < 1:
+        raise ValueError("max_new_tokens and check_every must be positive")
+    (B, P, _), K, dev = inputs_embeds.shape, num_beams, inputs_embeds.device
+    if prompt_lens is None:
+        prompt_lens = torch.full((B,), P, dtype=torch.int32, device=dev)
+    elif tuple(prompt_lens.shape) != (B,) or bool(((prompt_lens < 1) | (prompt_lens > P)).any()):
+        raise ValueError(f"prompt_lens must be [{B}], from 1 to {P}")
+    own = max_new_tokens // PAGE + 2  # pages behind the shared ones that a beam can hold
+    cache = PagedKVCache(B * K, P + max_new_tokens, decoder.kv_heads, decoder.head_dim, num_layers=decoder.num_layers,
+                         num_pages=B * (-(-P // PAGE) + K * own), device=dev)
+    prompts = cache.leaders(K)
+    prompts.extend(prompt_lens.to(dev))
+    logits = decoder(inputs_embeds, prompts, 1)
+    logits = logits.unsqueeze(1).expand(B, K, logits.shape[-1])  # beam 0 alone lives; the others' rows are not looked at
+    scores = torch.full((B, K), float("-inf"), device=dev)
+    scores[:, 0] = 0
+    history = torch.zeros((B, K, max_new_tokens), dtype=torch.int64, device=dev)
+    ended = torch.full((B, K), float("-inf"), device=dev)  # hypotheses, best first
+    ended_tokens, ended_lens = torch.zeros_like(history), torch.zeros((B, K), dtype=torch.int64, device=dev)
+    done = torch.zeros((B, 1), dtype=torch.bool, device=dev)
+    row = torch.arange(B, device=dev)[:, None]
+
+    def keep(new, tokens, lens):  # the best K of the old hypotheses and the new ones
+        nonlocal ended, ended_tokens, ended_lens
+        ended, at = torch.cat([ended, new], 1).sort(dim=1, descending=True, stable=True)
+        ended, at = ended[:, :K].contiguous(), at[:, :K]
+        ended_tokens = torch.cat([ended_tokens, tokens], 1)[row, at]
+        ended_lens = torch.cat([ended_lens, lens], 1).gather(1, at)
+
+    for t in range(max_new_tokens):
+        step = beam_select(logits, scores, eos_token_id)
+        if eos_token_id is not None:
+            new = step.cand_scores[:, :K] / float(t + 1) ** length_penalty
+            new = new.masked_fill((step.cand_tokens[:, :K] != eos_token_id) | done, float("-inf"))
+            keep(new, history[row, step.cand_parents[:, :K]], torch.full_like(ended_lens, t))
+            done = done | ((ended[:, -1:] > float("-inf")) & (step.scores[:, :1] / float(t + 1) ** length_penalty <= ended[:, -1:]))
+        history = reorder_states(history, step.parents)
+        history[:, :, t] = step.tokens
+        scores = step.scores
+        if t + 1 == max_new_tokens or (t % check_every == check_every - 1 and bool(done.all())):
+            break
+        cache.reorder(step.parents)
+        cache.extend(1)
+        logits = decoder(decoder.embed(step.tokens.view(-1)).unsqueeze(1), cache, K)
+    cache.check()
+    running = (scores / float(t + 1) ** length_penalty).masked_fill(done, float("-inf"))  # what ran to the end without one
+    keep(running, history, torch.full_like(ended_lens, t + 1))
+    tokens, lens = ended_tokens[:, 0].cpu(), ended_lens[:, 0].cpu()
+    return [tokens[b, :lens[b]].tolist() for b in range(B)], ended[:, 0]
 
 
 @torch.no_grad()

@@ -346,6 +346,8 @@ def test_attend_beams(dim, heads, group, beams, n, margins):
     q = torch.from_numpy(rng.standard_normal((S, n, heads * group, dim))).cuda().bfloat16()
     same_attention(c, o, q, beams=beams, margins=margins, name=f"{beams} beams, d {dim}, {heads} x {group}, {n} tokens")
     same_attention(c, o, q, beams=1, name="apart")
+    if beams * n * group <= 16:  # the same kernel: a row's bits do not depend on the rows that it is worked on with
+        assert torch.equal(c.attend(q, num_beams=beams), c.attend(q))
     par = rng.integers(0, beams, (3, beams))  # pages shared in no order
     c.reorder(torch.from_numpy(par).cuda())
     o.reorder(par)
@@ -586,3 +588,98 @@ def test_two_caches_on_two_streams():
     torch.cuda.synchronize()
     for t in range(10):
         assert torch.equal(outs[2 * t], ref[t]) and torch.equal(outs[2 * t + 1], ref[t])
+
+
+class TinyDecoder:
+    """One layer: attention over the cache and a residual, to logits."""
+
+    num_layers, kv_heads, head_dim, group = 1, 2, 64, 2
+
+    def __init__(self, vocab, width=48, seed=0):
+        g = _gen(seed)
+        r = lambda *shape: torch.randn(shape, generator=g, device="cuda") / math.sqrt(shape[0])  # noqa: E731
+        heads, d = self.kv_heads * self.group, self.head_dim
+        self.emb, self.wq, self.wk, self.wv = r(vocab, width) * 7, r(width, heads * d), r(width, self.kv_heads * d), r(width, self.kv_heads * d)
+        self.wo, self.wx = r(heads * d, vocab) * 6, r(width, vocab) * 3
+
+    def embed(self, tokens):
+        return self.emb[tokens]
+
+    def qkv(self, x):
+        S, n, _ = x.shape
+        return ((x @ w).bfloat16().view(S, n, -1, self.head_dim) for w in (self.wq, self.wk, self.wv))
+
+    def __call__(self, x, cache, num_beams):
+        q, k, v = self.qkv(x)
+        cache.write(k, v)
+        o = cache.attend(q, num_beams=num_beams).double()
+        y = o.flatten(2) @ self.wo.double() + x.double() @ self.wx.double()
+        last = (cache.lens - cache.starts).long() - 1
+        return y[torch.arange(len(y), device="cuda"), last].float()
+
+
+def plain_beam_search(dec, embeds, lens, K, steps, eos, penalty):
+    """One utterance at a time: hypotheses in Python lists, the oracle's selection, and a cache of its own for every beam, which
+    is copied whole when a beam continues another (no page is shared, nothing is reordered)."""
+    from asr_amd.decoding import PagedKVCache
+
+    def copied(c):
+        new = PagedKVCache(1, c.max_len, dec.kv_heads, dec.head_dim)
+        for name in ("kv", "exps", "table", "lens", "starts", "refs"):
+            getattr(new, name).copy_(getattr(c, name))
+        return new
+
+    out = []
+    for b in range(len(lens)):
+        caches = [PagedKVCache(1, int(lens[b]) + steps, dec.kv_heads, dec.head_dim)]
+        caches[0].extend(int(lens[b]))
+        logits = dec(embeds[b:b + 1, :lens[b]], caches[0], 1).expand(K, -1)
+        caches, scores, beams, ended, done = caches * K, np.array([[0.0] + [-np.inf] * (K - 1)]), [[]] * K, [], False
+        for t in range(steps):
+            s, tok, par, cs, ct, cp = od.select(logits.double().cpu().numpy()[None], scores, eos)
+            for j in range(K):
+                if ct[0, j] == eos and not done:
+                    ended.append((cs[0, j] / (t + 1) ** penalty, beams[cp[0, j]]))
+            ended = sorted(ended, key=lambda e: -e[0])[:K]
+            done = done or (len(ended) == K and s[0, 0] / (t + 1) ** penalty <= ended[-1][0])
+            beams = [beams[par[0, j]] + [int(tok[0, j])] for j in range(K)]
+            scores = s
+            if t + 1 == steps or done:
+                break
+            caches = [copied(caches[par[0, j]]) for j in range(K)]
+            for c in caches:
+                c.extend(1)
+            logits = torch.cat([dec(dec.embed(torch.tensor([[tok[0, j]]], device="cuda")), c, 1) for j, c in enumerate(caches)])
+        if not done:
+            ended += [(scores[0, j] / (t + 1) ** penalty, beams[j]) for j in range(K)]
+        best = max(ended, key=lambda e: e[0])
+        out.append((best[1], best[0]))
+    return out
+
+
+@pytest.mark.parametrize("K,penalty,steps", [(1, 1.0, 20), (3, 1.0, 40), (5, 0.0, 30), (4, 2.0, 70)])
+def test_beam_generate_follows_a_plain_beam_search(K, penalty, steps):
+    from asr_amd.evaluation import beam_generate
+
+    dec = TinyDecoder(37, seed=K)
+    embeds = torch.randn((3, 90, 48), generator=_gen(50 + K), device="cuda")
+    lens = torch.tensor([90, 13, 64], device="cuda")
+    tokens, scores = beam_generate(dec, embeds, num_beams=K, max_new_tokens=steps, eos_token_id=4, length_penalty=penalty, prompt_lens=lens)
+    for b, (want, score) in enumerate(plain_beam_search(dec, embeds, lens.tolist(), K, steps, 4, penalty)):
+        assert tokens[b] == want, (b, tokens[b], want)
+        assert abs(float(scores[b]) - score) <= 1e-5 * steps  # float32 logits and scores in every step
+    assert any(len(t) < steps for t in tokens) or K == 1
+
+
+def test_beam_generate_refusals():
+    from asr_amd.evaluation import beam_generate
+
+    dec, x = TinyDecoder(9), torch.zeros((2, 5, 48), device="cuda")
+    for kw in (dict(max_new_tokens=0), dict(check_every=0), dict(num_beams=17), dict(prompt_lens=torch.tensor([1, 6], device="cuda")),
+               dict(prompt_lens=torch.tensor([0, 2], device="cuda"))):
+        with pytest.raises(ValueError):
+            beam_generate(dec, x, **kw)
+    with pytest.raises(ValueError):
+        beam_generate(dec, x[0])
+    tokens, scores = beam_generate(dec, x, num_beams=2, max_new_tokens=3)  # no end token
+    assert [len(t) for t in tokens] == [3, 3] and bool(scores.isfinite().all())

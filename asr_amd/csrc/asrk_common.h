@@ -39,10 +39,10 @@ __device__ __forceinline__ float gelu_erf(float x) {
     return fmaf(fabsf(h), fmaf(-p, e, 1.0f), h);
 }
 
-// The same for two values at once on the packed fp32 pipe (v_pk_fma_f32 / v_pk_mul_f32: two lanes' worth of work per
-// issue; an epilogue is pure VALU, there is no MFMA beside it to disturb).  Returns 2 * gelu(x) so that the caller can
-// fold the 0.5 into its own scale.  11 packed + 2 plain + 4 transcendental issues per pair: 42 cycles per value against
-// 68 for gelu_erf.  Coefficients negated so that erf = 1 + q e needs no sign flip.
+// The same for two values at once.  Returns 2 * gelu(x) so that the caller can fold the 0.5 into its own scale.  As packed
+// fp32 instructions 11 + 2 plain + 4 transcendental issues per pair, 42 cycles per value against 68 for gelu_erf; the
+// build compiles them to plain ones (see the Makefile: the same bits, and a whole encoder pass within 0.3 %).
+// Coefficients negated so that erf = 1 + q e needs no sign flip.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2_t gelu_erf_x2(f32x2_t x) {
     f32x2_t ax;

@@ -12,7 +12,7 @@ for f in asrk_*.hip; do
   for g in "$@"; do
     if [ "$g" = "$f" ]; then
       o=build/var_$name/${f%.hip}.o
-      /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-function $flags $( [ $f = asrk_logmel.hip ] && echo -fno-slp-vectorize ) -c $f -o $o &
+      /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-function $flags $( [ $f = asrk_logmel.hip ] && echo -fno-slp-vectorize ) -c $f -o $o &
     fi
   done
   objs="$objs $o"

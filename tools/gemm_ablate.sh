@@ -6,7 +6,7 @@
 set -e
 cd "$(dirname "$0")/../asr_amd/csrc"
 for n in ${ABL:-1 2 3 4 8 12}; do
-  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -DASRK_DIAG -DASRK_STAMPS -DASRK_ABLATE=$n -c asrk_gemm256p.hip -o build/stamps/abl$n.o &
+  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -DASRK_DIAG -DASRK_STAMPS -DASRK_ABLATE=$n -c asrk_gemm256p.hip -o build/stamps/abl$n.o &
 done
 wait
 for n in ${ABL:-1 2 3 4 8 12}; do

@@ -13,8 +13,7 @@
 namespace {
 
 constexpr int SEL_WAVES = 4;
-constexpr int SEL_EPT = 32;                          // logits per lane
-constexpr int SEL_CHUNK = SEL_WAVES * 64 * SEL_EPT;  // logits per workgroup
+constexpr int SEL_CHUNK = 8192;  // logits per workgroup: 32 per lane, or twice that
 constexpr int SEL_MAX_BEAMS = 16;
 constexpr int SEL_MAX_N = 2 * SEL_MAX_BEAMS;
 constexpr int SEL_MAX_LISTS = 2048;
@@ -61,9 +60,9 @@ constexpr int sel_lanes(int n) { return n + 8; }  // lanes of a workgroup whose 
 // the chunk's n-th best value, and only those lanes can hold values that count.  Bisection finds one with n .. n + 8 such
 // lanes in a few steps, a compare and a bit count per wave's worth of lanes; every wave does it for itself on all 256.
 // Where equal values leave no such threshold it falls back to ranking the lane maxima by (value, ~word), which are all
-// different.  Either way at most sel_lanes(n) lanes of 32 keys reach LDS, for any input (with random logits about n + 6
+// different.  Either way at most sel_lanes(n) lanes of 32 (64) keys reach LDS, for any input (with random logits about n + 6
 // keys do).
-template <class T>
+template <class T, int SEL_EPT>  // logits per lane
 __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ logits, int64_t ld, int V, int n,
                                                          uint64_t* __restrict__ keys, float2* __restrict__ stats) {
     constexpr int VEC = SelVec<T>::N;
@@ -338,13 +337,20 @@ __global__ __launch_bounds__(256) void reorder_rows_kernel(const T* __restrict__
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < units; i += (int64_t)gridDim.x * 256) dst[i] = src[i];
 }
 
-int sel_chunks(int V) { return (int)(((int64_t)V + SEL_CHUNK - 1) / SEL_CHUNK); }
+int sel_chunks(int V, int chunk) { return (int)(((int64_t)V + chunk - 1) / chunk); }
+
+// bf16 rows are bound by instructions, and what a workgroup does besides its logits halves with twice as many of them; so
+// where there are workgroups for more than one round of the card (8 on each of 256 CUs), it takes them: 64 x 5 rows of
+// 51865 words 17.1 -> 14.4 us.  fp32 rows are bound by memory: 32 x 8 rows of 128001 words 27.3 -> 28.8 us, not taken.
+int sel_chunk(int dtype, int64_t rows, int V) {
+    return dtype == ASRK_BF16 && rows * sel_chunks(V, SEL_CHUNK) > 2048 ? 2 * SEL_CHUNK : SEL_CHUNK;
+}
 
 }  // namespace
 
 extern "C" size_t asrk_beam_select_workspace_bytes(int B, int K, int V) {
     if (B <= 0 || K <= 0 || K > SEL_MAX_BEAMS || V < 2) return 0;
-    return (size_t)B * K * sel_chunks(V) * (2 * K * sizeof(uint64_t) + SEL_WAVES * sizeof(float2));
+    return (size_t)B * K * sel_chunks(V, SEL_CHUNK) * (2 * K * sizeof(uint64_t) + SEL_WAVES * sizeof(float2));
 }
 
 extern "C" int asrk_beam_select(const void* logits, int dtype, int64_t ld, const float* scores, int B, int K, int V, int64_t eos,
@@ -355,7 +361,7 @@ extern "C" int asrk_beam_select(const void* logits, int dtype, int64_t ld, const
     if (dtype != ASRK_F32 && dtype != ASRK_BF16) return ASRK_ERR_UNSUPPORTED;
     if (B <= 0 || K <= 0 || K > SEL_MAX_BEAMS || V < 2 || ld < V || (int64_t)B * K > 65535 || (int64_t)K * V > 0x7fffffff)
         return ASRK_ERR_SHAPE;
-    const int chunks = sel_chunks(V);
+    const int chunk = sel_chunk(dtype, (int64_t)B * K, V), chunks = sel_chunks(V, chunk);
     if (K * chunks > SEL_MAX_LISTS) return ASRK_ERR_SHAPE;
     if ((uintptr_t)logits % (dtype == ASRK_F32 ? 4 : 2)) return ASRK_ERR_ALIGN;
     if ((uintptr_t)ws & 15) return ASRK_ERR_ALIGN;
@@ -363,13 +369,14 @@ extern "C" int asrk_beam_select(const void* logits, int dtype, int64_t ld, const
     uint64_t* keys = (uint64_t*)ws;
     float2* stats = (float2*)(keys + (size_t)B * K * chunks * 2 * K);
     hipStream_t st = (hipStream_t)stream;
-    const size_t lds = (size_t)sel_lanes(2 * K) * SEL_EPT * sizeof(uint64_t);  // 10 KiB at most
+    const size_t lds = (size_t)sel_lanes(2 * K) * (chunk / 256) * sizeof(uint64_t);  // 20 KiB at most
+    const dim3 grid(chunks, B * K);
     if (dtype == ASRK_F32)
-        hipLaunchKernelGGL(beam_chunk_kernel<float>, dim3(chunks, B * K), dim3(256), lds, st, (const float*)logits, ld, V, 2 * K, keys,
-                           stats);
+        hipLaunchKernelGGL((beam_chunk_kernel<float, 32>), grid, dim3(256), lds, st, (const float*)logits, ld, V, 2 * K, keys, stats);
+    else if (chunk == SEL_CHUNK)
+        hipLaunchKernelGGL((beam_chunk_kernel<bf16_t, 32>), grid, dim3(256), lds, st, (const bf16_t*)logits, ld, V, 2 * K, keys, stats);
     else
-        hipLaunchKernelGGL(beam_chunk_kernel<bf16_t>, dim3(chunks, B * K), dim3(256), lds, st, (const bf16_t*)logits, ld, V, 2 * K,
-                           keys, stats);
+        hipLaunchKernelGGL((beam_chunk_kernel<bf16_t, 64>), grid, dim3(256), lds, st, (const bf16_t*)logits, ld, V, 2 * K, keys, stats);
     hipLaunchKernelGGL(beam_join_kernel, dim3(B), dim3(JOIN_T), 0, st, keys, stats, scores, K, V, chunks, 2 * K, eos, out_scores,
                        out_tokens, out_parents, cand_scores, cand_tokens, cand_parents);
     return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;

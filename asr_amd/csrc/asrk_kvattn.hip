@@ -33,7 +33,7 @@ struct AttnArgs {
     bf16_t* out;
     float* part_o;   // [splits][S n Hq][D]
     float2* part_ml; // [splits][S n Hq]
-    int64_t seq_ld, row_ld, head_ld, layer;
+    int64_t seq_ld, row_ld, head_ld, layer, rows;  // rows: S n Hq
     int n, group, beams, splits;  // new tokens, query heads per key/value head
     float c;
 };
@@ -77,80 +77,241 @@ __device__ __forceinline__ int wave_imax(int v) {
     return v;
 }
 
+// Column y of a set of sequences: beam, new token, query head.
+struct Columns {
+    const AttnArgs& a;
+    int set, h, H, per_seq, columns;
+    __device__ __forceinline__ Columns(const asrk_kv_cache& c, const AttnArgs& args, int set_)
+        : a(args), set(set_), h(blockIdx.y), H(c.kv_heads), per_seq(args.n * args.group), columns(args.beams * per_seq) {}
+    __device__ __forceinline__ void split(int y, int& b, int& i, int& j) const {
+        b = a.beams == 1 ? 0 : (int)((unsigned)y / (unsigned)per_seq);
+        const unsigned in = (unsigned)(y - b * per_seq);
+        i = a.n == 1 ? 0 : (int)(in / (unsigned)a.group);
+        j = (int)in - i * a.group;
+    }
+    __device__ __forceinline__ int64_t row_of(int y) const {  // of out, in units of D
+        int b, i, j;
+        split(y, b, i, j);
+        return (((int64_t)set * a.beams + b) * a.n + i) * (int64_t)(H * a.group) + h * a.group + j;
+    }
+};
+
+// What a lane holds of its CT columns: q as the second operand (16 consecutive d's per pair of steps), the beam, the number
+// of tokens seen; the largest such number of the wave.
+template <int D, int CT>
+struct Queries {
+    bf16x8 q[CT][D / 32];
+    int limit[CT], beam[CT], most;
+    __device__ __forceinline__ void load(const asrk_kv_cache& c, const Columns& cs, int first_col, int col, int g) {
+        const int top = c.max_pages * ASRK_KV_PAGE;
+        most = 0;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const int x = first_col + 16 * t + col;
+            beam[t] = 0;
+            limit[t] = NO_COLUMN;
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q[t][s][e] = (bf16_t)0.f;
+            if (x < cs.columns) {
+                int b, i, j;
+                cs.split(x, b, i, j);
+                const int64_t seq = (int64_t)cs.set * cs.a.beams + b;
+                const int start = c.starts[seq * c.seq_stride], fresh = c.lens[seq * c.seq_stride] - start;
+                beam[t] = b;
+                limit[t] = i >= fresh ? 0 : (start + i + 1 < top ? start + i + 1 : top);
+                most = limit[t] > most ? limit[t] : most;
+                const bf16_t* p = cs.a.q + seq * cs.a.seq_ld + (int64_t)i * cs.a.row_ld + (int64_t)(cs.h * cs.a.group + j) * cs.a.head_ld + 16 * g;
+#pragma unroll
+                for (int s = 0; s < D / 64; ++s) {
+                    q[t][2 * s] = *reinterpret_cast<const bf16x8*>(p + 64 * s);
+                    q[t][2 * s + 1] = *reinterpret_cast<const bf16x8*>(p + 64 * s + 8);
+                }
+            }
+        }
+        most = __builtin_amdgcn_readfirstlane(wave_imax(most));
+    }
+    // Of page p, for the beams `with`: tokens seen by each column; whether all see all of it, and whether any sees any.
+    __device__ __forceinline__ bool see(int p, uint64_t with, int* seen, bool& whole) const {
+        int all = ASRK_KV_PAGE, some = 0;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const int s = limit[t] - p * ASRK_KV_PAGE;
+            const bool takes = (with >> beam[t]) & 1;
+            seen[t] = limit[t] == NO_COLUMN || (takes && s > ASRK_KV_PAGE) ? ASRK_KV_PAGE : (takes && s > 0 ? s : 0);
+            all = seen[t] < all ? seen[t] : all;
+            some = seen[t] > some && limit[t] != NO_COLUMN ? seen[t] : some;
+        }
+        whole = __all(all == ASRK_KV_PAGE);
+        return __any(some > 0);
+    }
+};
+
+// The work on a set of sequences, page by page: beams whose tables agree on a page take it together.
+struct Item {
+    int page, p;  // -1: no more; the p-th page of its sequences
+    uint64_t with;
+};
+struct Pages {
+    const int* table;  // of beam `lane`
+    int beams, max_pages, num_pages, lane, at_p, step, item_p, mine, coming;
+    uint64_t left;
+    __device__ __forceinline__ Pages(const asrk_kv_cache& c, int beams_, int set, int first, int step_)
+        : beams(beams_), max_pages(c.max_pages), num_pages(c.num_pages), lane(threadIdx.x & 63), at_p(first), step(step_), item_p(0),
+          mine(-1), left(0) {
+        table = c.table + ((int64_t)set * beams + lane) * c.seq_stride * max_pages;
+        coming = number(first);
+    }
+    __device__ __forceinline__ int number(int p) const { return lane < beams && p < max_pages ? table[p] : -1; }
+    __device__ __forceinline__ Item next(int pages) {
+        while (!left) {
+            if (at_p >= pages) return Item{-1, 0, 0};
+            mine = coming;
+            item_p = at_p;
+            at_p += step;
+            coming = number(at_p);  // on its way a page ahead
+            left = __ballot(mine >= 0 && mine < num_pages);
+        }
+        const int page = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+        const uint64_t with = __ballot(mine == page) & left;
+        left &= ~with;
+        return Item{page, item_p, with};
+    }
+};
+
+// Loads go through a descriptor of the page: one register of lane offset, the rest in the instruction.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rows(const char* layer, int64_t at, int D) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(uniform_ptr(layer + at * (2 * ASRK_KV_PAGE * D))), 0, 2 * ASRK_KV_PAGE * D,
+                                             0x00020000);
+}
+
+// Bytes of the lane's 16 tokens that lie before token `last` of the page (behind the last token the page may hold anything).
+__device__ __forceinline__ u32x4 keep_before(int last, int g) {
+    u32x4 mask;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int keep = last - 16 * g - 4 * w;
+        mask[w] = (uint32_t)((1ull << (8 * (keep < 0 ? 0 : (keep > 4 ? 4 : keep)))) - 1);
+    }
+    return mask;
+}
+// Tokens that the longest of the beams `with` has of page p.
+__device__ __forceinline__ int tokens_held(const asrk_kv_cache& c, int set, int beams, uint64_t with, int p) {
+    const int lane = threadIdx.x & 63;
+    const int len = lane < beams && ((with >> lane) & 1) ? c.lens[((int64_t)set * beams + lane) * c.seq_stride] : 0;
+    const int held = __builtin_amdgcn_readfirstlane(wave_imax(len)) - p * ASRK_KV_PAGE;
+    return held < 0 ? 0 : (held > ASRK_KV_PAGE ? ASRK_KV_PAGE : held);
+}
+
+// Scores of one page to weights.  The reference follows the maximum only when that has grown by more than 2^8: up to there
+// the weights stay within f16, at the same relative precision, and o and the sum need no rescaling.
+template <int CT, int DT>
+__device__ __forceinline__ void weigh(f32x4 (*sc)[4], const int* seen, bool whole, int g, float scale, int up, int unit, float* m, f32x4* l,
+                                      f32x4 (*o)[DT], f16x8 (*pf)[2]) {
+    const float shrink = pow2(unit - up);
+#pragma unroll
+    for (int x = 0; x < CT; ++x) {
+        if (!whole) {
+            KEEP_BRANCH();
+            const int mine = seen[x] - 16 * g;  // of the lane's 16 tokens
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[x][t][i] = 4 * t + i < mine ? sc[x][t][i] : NEG_INF;
+        }
+        float top = NEG_INF;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[x][t][i]);
+        const float now = groups_max(top) * scale;  // scale > 0
+        if (__any(now > m[x] + 8.f) || up != unit) {
+            KEEP_BRANCH();
+            const float to = now > m[x] + 8.f ? now : m[x];  // by the column alone: its bits do not depend on its neighbours
+            const float back = to > NEG_INF ? __builtin_amdgcn_exp2f(m[x] - to) : 0.f;
+            m[x] = to;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[x][i] *= back;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[x][d] *= back * shrink;
+        }
+        const float ref = m[x] > NEG_INF ? m[x] : 0.f;  // nothing seen yet: every weight is 0
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const f32x2_t w = {__builtin_amdgcn_exp2f(fmaf(sc[x][t][i], scale, -ref)),
+                                   __builtin_amdgcn_exp2f(fmaf(sc[x][t][i + 1], scale, -ref))};
+                const f16x2 h = __builtin_convertvector(w, f16x2);  // to nearest
+                pf[x][t >> 1][4 * (t & 1) + i] = h[0];
+                pf[x][t >> 1][4 * (t & 1) + i + 1] = h[1];
+            }
+    }
+}
+
+// The sum of the weights as they are used: a product with ones, all four rows of a lane are the column's sum.
+template <int CT>
+__device__ __forceinline__ void add_weights(const f16x8 (*pf)[2], f32x4* l) {
+    const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+#pragma unroll
+    for (int x = 0; x < CT; ++x)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) l[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[x][u], l[x], 0, 0, 0);
+}
+
+// A page whose values hold a NaN (rare: the page says so).  0 * NaN must not reach columns that do not see its token, so the
+// NaNs were made zeros for the product; here what a product of the 0/1 patterns (is a NaN, is seen) says becomes NaN.
+template <int CT, int DT, class Load>
+__device__ __forceinline__ void mark_nans(Load&& raw_value, const int* seen, int g, f32x4 (*o)[DT]) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+        __builtin_amdgcn_sched_barrier(0);  // one tile at a time: this path must not cost the other one registers
+        const u32x4 raw = raw_value(d);
+#pragma unroll
+        for (int x = 0; x < CT; ++x) {
+            f32x4 hit{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                f16x8 sees;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sees[i] = 16 * g + 8 * u + i < seen[x] ? (_Float16)1.f : (_Float16)0.f;
+                const f16x8 is = v8(nan_bytes(raw[2 * u]) & 0x38383838u, nan_bytes(raw[2 * u + 1]) & 0x38383838u, 1.f);  // 0x38 is 1
+                hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees, hit, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[x][d][i] = hit[i] > 0.f ? __builtin_nanf("") : o[x][d][i];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // Waves per SIMD that the registers are cut for: as many as hold a page, q, o and the scores without spilling in the loop.
 // (D 64, 1 tile: 4; with 3, 64 x 5 beams take 24.5 us instead of 19.7.  D 128, 1 tile: 2; with 3 it spills and 1.2 GB of
 // cache take 228 us instead of 204.)
 constexpr int occupancy(int D, int CT) { return D == 64 ? (CT == 1 ? 4 : 3) : 2; }
 
-// CT column tiles of 16 per wave.  OWN_COLUMNS: every wave has columns of its own and walks all pages (prompts, where
-// columns abound); otherwise the W waves share the columns and deal the pages among them (and among the splits).
-template <int D, int CT, int W, bool OWN_COLUMNS>
+// Few columns (single tokens): the W waves of a workgroup share CT tiles of 16 and deal the pages among them, and among
+// the splits.  A wave takes a page straight into registers; the next page's keys are loaded over this one's as soon as the
+// scores are done, its values as soon as they are used.
+template <int D, int CT, int W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(occupancy(D, CT), occupancy(D, CT))))
 void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     constexpr int KS = D / 64;   // 16-byte pieces of a key row per lane
     constexpr int DT = D / 16;   // tiles of 16 d
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int H = c.kv_heads, M = c.max_pages;
-    const int h = blockIdx.y;
-    const int per_seq = a.n * a.group;          // columns of a sequence
-    const int columns = a.beams * per_seq;
-    const int chunks = (columns + 16 * CT * (OWN_COLUMNS ? W : 1) - 1) / (16 * CT * (OWN_COLUMNS ? W : 1));
-    // The last rows of every prompt first: they see the most, and what is left for the end is short.
-    const int sets = c.num_seqs / a.beams, set = blockIdx.z % sets, chunk = chunks - 1 - blockIdx.z / sets;
-    const int first_col = (OWN_COLUMNS ? chunk * W + wave : chunk) * 16 * CT;
-
+    const int sets = c.num_seqs / a.beams, set = blockIdx.z % sets;
+    const Columns cs(c, a, set);
+    const int first_col = blockIdx.z / sets * 16 * CT;
     // The pages of a wave: by its number alone, so that their numbers are on the way before the lengths are known.
-    const int p0 = OWN_COLUMNS ? 0 : blockIdx.x * W + wave, step = OWN_COLUMNS ? 1 : a.splits * W;
-    const int* table = c.table + ((int64_t)set * a.beams + lane) * c.seq_stride * M;  // of beam `lane`
-    auto page_of = [&](int p) __attribute__((always_inline)) { return lane < a.beams && p < M ? table[p] : -1; };
-    int coming = page_of(p0);
-
-    auto split = [&](int y, int& b, int& i, int& j) __attribute__((always_inline)) {  // column: beam, new token, query head
-        b = a.beams == 1 ? 0 : (int)((unsigned)y / (unsigned)per_seq);
-        const unsigned in = (unsigned)(y - b * per_seq);
-        i = a.n == 1 ? 0 : (int)(in / (unsigned)a.group);
-        j = (int)in - i * a.group;
-    };
-    auto row_of = [&](int y) __attribute__((always_inline)) {  // of q and out, in units of D
-        int b, i, j;
-        split(y, b, i, j);
-        return (((int64_t)set * a.beams + b) * a.n + i) * (int64_t)(H * a.group) + h * a.group + j;
-    };
-    // ---- this lane's columns: beam, tokens seen, row of q
-    int limit[CT], beam[CT];
-    bf16x8 qf[CT][2 * KS];
-    int most = 0;
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        const int x = first_col + 16 * t + col;
-        int b, i, j;
-        split(x, b, i, j);
-        beam[t] = 0;
-        limit[t] = NO_COLUMN;
-#pragma unroll
-        for (int s = 0; s < 2 * KS; ++s)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) qf[t][s][e] = (bf16_t)0.f;
-        if (x < columns) {
-            const int64_t seq = (int64_t)set * a.beams + b;
-            const int start = c.starts[seq * c.seq_stride], fresh = c.lens[seq * c.seq_stride] - start;
-            beam[t] = b;
-            limit[t] = i >= fresh ? 0 : (start + i + 1 < M * ASRK_KV_PAGE ? start + i + 1 : M * ASRK_KV_PAGE);
-            most = limit[t] > most ? limit[t] : most;
-            const bf16_t* q = a.q + seq * a.seq_ld + (int64_t)i * a.row_ld + (int64_t)(h * a.group + j) * a.head_ld + 16 * g;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                qf[t][2 * s] = *reinterpret_cast<const bf16x8*>(q + 64 * s);
-                qf[t][2 * s + 1] = *reinterpret_cast<const bf16x8*>(q + 64 * s + 8);
-            }
-        }
-    }
-    most = __builtin_amdgcn_readfirstlane(wave_imax(most));
+    Pages work(c, a.beams, set, blockIdx.x * W + wave, a.splits * W);
+    Queries<D, CT> qs;
+    qs.load(c, cs, first_col, col, g);
+    const int pages = (qs.most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
 
     f32x4 o[CT][DT], l[CT];
     float m[CT];
-    const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         m[t] = NEG_INF;
@@ -160,37 +321,9 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     }
     int unit = ASRK_KV_EXP_MIN;  // o is in units of 2^unit
 
-    const int pages = (most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
-    const char* layer = (const char*)c.kv + a.layer * c.num_pages * H * (int64_t)(2 * ASRK_KV_PAGE * D);
-    const int* exps = (const int*)c.exps + a.layer * c.num_pages * H;
+    const char* layer = (const char*)c.kv + a.layer * c.num_pages * cs.H * (int64_t)(2 * ASRK_KV_PAGE * D);
+    const int* exps = (const int*)c.exps + a.layer * c.num_pages * cs.H;
     const uint32_t k_at = (16 * (col >> 2) + (col & 3)) * D + 16 * g, v_at = col * ASRK_KV_PAGE + 16 * g;  // this lane's bytes
-
-    // The wave's work, page by page: beams whose tables agree on a page take it together.
-    struct Item {
-        int page, p;  // -1: no more; the p-th page of its sequences
-        uint64_t with;
-    };
-    int at_p = p0, item_p = 0, mine = -1;
-    uint64_t left = 0;
-    auto advance = [&]() __attribute__((always_inline)) -> Item {
-        while (!left) {
-            if (at_p >= pages) return Item{-1, 0, 0};
-            mine = coming;
-            item_p = at_p;
-            at_p += step;
-            coming = page_of(at_p);
-            left = __ballot(mine >= 0 && mine < c.num_pages);
-        }
-        const int page = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-        const uint64_t with = __ballot(mine == page) & left;
-        left &= ~with;
-        return Item{page, item_p, with};
-    };
-    // Loads go through a descriptor of the page: one register of lane offset, the rest in the instruction.
-    auto rows_of = [&](int page) __attribute__((always_inline)) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(uniform_ptr(layer + ((int64_t)page * H + h) * (2 * ASRK_KV_PAGE * D))), 0,
-                                                 2 * ASRK_KV_PAGE * D, 0x00020000);
-    };
     u32x4 kr[4][KS], vr[DT];
     auto load_keys = [&](__amdgpu_buffer_rsrc_t rows) __attribute__((always_inline)) {
 #pragma unroll
@@ -201,164 +334,75 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     auto load_value = [&](__amdgpu_buffer_rsrc_t rows, int d) __attribute__((always_inline)) {
         return __builtin_amdgcn_raw_buffer_load_b128(rows, v_at + 16 * d * ASRK_KV_PAGE, ASRK_KV_PAGE * D, 0);
     };
-    Item item = advance();
-    __amdgpu_buffer_rsrc_t rows = rows_of(item.page < 0 ? 0 : item.page);
+    Item item = work.next(pages);
+    int64_t at = (int64_t)(item.page < 0 ? 0 : item.page) * cs.H + cs.h;
+    __amdgpu_buffer_rsrc_t rows = page_rows(layer, at, D);
     int e_next = 0;
     if (item.page >= 0) {
-        e_next = exps[(int64_t)item.page * H + h];
+        e_next = exps[at];
         load_keys(rows);
 #pragma unroll
         for (int d = 0; d < DT; ++d) vr[d] = load_value(rows, d);
     }
     while (item.page >= 0) {
-        // The next page's keys are loaded over this one's as soon as the scores are done, its values as soon as they are used.
-        const Item following = advance();
-        const __amdgpu_buffer_rsrc_t rows_next = rows_of(following.page < 0 ? 0 : following.page);
-        {
-            const int p = item.p;
-            const uint64_t with = item.with;
-            const int e = __builtin_amdgcn_readfirstlane(e_next);
-            if (following.page >= 0) e_next = exps[(int64_t)following.page * H + h];
-            // ---- which columns see how much of it
-            int seen[CT];
-            int all = ASRK_KV_PAGE, some = 0;
-#pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                const int s = limit[t] - p * ASRK_KV_PAGE;
-                const bool takes = (with >> beam[t]) & 1;
-                seen[t] = limit[t] == NO_COLUMN || (takes && s > ASRK_KV_PAGE) ? ASRK_KV_PAGE : (takes && s > 0 ? s : 0);
-                all = seen[t] < all ? seen[t] : all;
-                some = seen[t] > some && limit[t] != NO_COLUMN ? seen[t] : some;
-            }
-            const bool whole = __all(all == ASRK_KV_PAGE);
+        const Item following = work.next(pages);
+        at = (int64_t)(following.page < 0 ? 0 : following.page) * cs.H + cs.h;
+        const __amdgpu_buffer_rsrc_t rows_next = page_rows(layer, at, D);
+        const int e = __builtin_amdgcn_readfirstlane(e_next);
+        if (following.page >= 0) e_next = exps[at];
+        int seen[CT];
+        bool whole;
+        qs.see(item.p, item.with, seen, whole);
 
-            const float ks = pow2((int8_t)e);
-            const int ev = (int8_t)(e >> 8);
-            // ---- scores
-            f32x4 sc[CT][4];
+        const float ks = pow2((int8_t)e);
+        const int ev = (int8_t)(e >> 8), up = ev > unit ? ev : unit;
+        f32x4 sc[CT][4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 4; ++t) {
 #pragma unroll
-                for (int x = 0; x < CT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int x = 0; x < CT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const bf16x8 k0 = k8(kr[t][s][0], kr[t][s][1], ks), k1 = k8(kr[t][s][2], kr[t][s][3], ks);
+            for (int s = 0; s < KS; ++s) {
+                const bf16x8 k0 = k8(kr[t][s][0], kr[t][s][1], ks), k1 = k8(kr[t][s][2], kr[t][s][3], ks);
 #pragma unroll
-                    for (int x = 0; x < CT; ++x) {
-                        sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[x][2 * s], sc[x][t], 0, 0, 0);
-                        sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[x][2 * s + 1], sc[x][t], 0, 0, 0);
-                    }
-                }
-            }
-            if (following.page >= 0) load_keys(rows_next);
-            // ---- weights
-            // The reference follows the maximum only when that has grown by more than 2^8: up to there the weights stay
-            // within f16, at the same relative precision, and o and the sum need no rescaling.
-            const int up = ev > unit ? ev : unit;
-            const float shrink = pow2(unit - up);
-            f16x8 pf[CT][2];
-#pragma unroll
-            for (int x = 0; x < CT; ++x) {
-                if (!whole) {
-                    KEEP_BRANCH();
-                    const int mine = seen[x] - 16 * g;  // of the lane's 16 tokens
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[x][t][i] = 4 * t + i < mine ? sc[x][t][i] : NEG_INF;
-                }
-                float top = NEG_INF;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[x][t][i]);
-                const float now = groups_max(top) * a.c;  // c > 0
-                if (__any(now > m[x] + 8.f) || up != unit) {
-                    KEEP_BRANCH();
-                    const float to = now > m[x] + 8.f ? now : m[x];  // by the column alone: its bits do not depend on its neighbours
-                    const float back = to > NEG_INF ? __builtin_amdgcn_exp2f(m[x] - to) : 0.f;
-                    m[x] = to;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) l[x][i] *= back;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) o[x][d] *= back * shrink;
-                }
-                const float ref = m[x] > NEG_INF ? m[x] : 0.f;  // nothing seen yet: every weight is 0
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        const f32x2_t w = {__builtin_amdgcn_exp2f(fmaf(sc[x][t][i], a.c, -ref)),
-                                           __builtin_amdgcn_exp2f(fmaf(sc[x][t][i + 1], a.c, -ref))};
-                        const f16x2 h = __builtin_convertvector(w, f16x2);  // to nearest
-                        pf[x][t >> 1][4 * (t & 1) + i] = h[0];
-                        pf[x][t >> 1][4 * (t & 1) + i + 1] = h[1];
-                    }
-            }
-            unit = up;
-            const float vs = pow2(ev - up);
-            if (!whole) {  // bytes behind the last token seen by anyone may be anything
-                KEEP_BRANCH();
-                const int last = wave_imax(some) - 16 * g;
-                uint32_t mask[4];
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int keep = last - 4 * w < 0 ? 0 : (last - 4 * w > 4 ? 4 : last - 4 * w);
-                    mask[w] = (uint32_t)((1ull << (8 * keep)) - 1);
-                }
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        vr[d][w] &= mask[w];
-                    }
-            }
-            // The values may hold a NaN (rare: the page says so), and 0 * NaN must not reach columns that do not see its
-            // token.  The NaNs become zeros, and below, what a product of the 0/1 patterns (is a NaN, is seen) says becomes NaN.
-            const bool odd = __builtin_expect((e >> 16) & 1, 0);
-            if (odd) {
-                KEEP_BRANCH();
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) vr[d][w] &= ~nan_bytes(vr[d][w]);
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const f16x8 v = v8(vr[d][2 * u], vr[d][2 * u + 1], vs);
-#pragma unroll
-                    for (int x = 0; x < CT; ++x) o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[x][u], o[x][d], 0, 0, 0);
-                }
-            // the sum of the weights as they are used: a product with ones, all four rows of a lane are the column's sum
-#pragma unroll
-            for (int x = 0; x < CT; ++x)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) l[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[x][u], l[x], 0, 0, 0);
-            if (odd) {
-#pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    __builtin_amdgcn_sched_barrier(0);  // one tile at a time: this path must not cost the other one registers
-                    const u32x4 raw = load_value(rows, d);
-#pragma unroll
-                    for (int x = 0; x < CT; ++x) {
-                        f32x4 hit{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            f16x8 sees;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) sees[i] = 16 * g + 8 * u + i < seen[x] ? (_Float16)1.f : (_Float16)0.f;
-                            const f16x8 is = v8(nan_bytes(raw[2 * u]) & 0x38383838u, nan_bytes(raw[2 * u + 1]) & 0x38383838u, 1.f);  // 0x38 is 1
-                            hit = __builtin_amdgcn_mfma_f32_16x16x32_f16(is, sees, hit, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[x][d][i] = hit[i] > 0.f ? __builtin_nanf("") : o[x][d][i];
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+                for (int x = 0; x < CT; ++x) {
+                    sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qs.q[x][2 * s], sc[x][t], 0, 0, 0);
+                    sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qs.q[x][2 * s + 1], sc[x][t], 0, 0, 0);
                 }
             }
         }
+        if (following.page >= 0) load_keys(rows_next);
+        f16x8 pf[CT][2];
+        weigh<CT, DT>(sc, seen, whole, g, a.c, up, unit, m, l, o, pf);
+        unit = up;
+        const float vs = pow2(ev - up);
+        if (!whole) {
+            KEEP_BRANCH();
+            int last = 0;  // token seen by any column
+#pragma unroll
+            for (int x = 0; x < CT; ++x) last = seen[x] > last && qs.limit[x] != NO_COLUMN ? seen[x] : last;
+            const u32x4 mask = keep_before(wave_imax(last), g);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) vr[d] &= mask;
+        }
+        const bool odd = __builtin_expect((e >> 16) & 1, 0);
+        if (odd) {
+            KEEP_BRANCH();
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) vr[d][w] &= ~nan_bytes(vr[d][w]);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const f16x8 v = v8(vr[d][2 * u], vr[d][2 * u + 1], vs);
+#pragma unroll
+                for (int x = 0; x < CT; ++x) o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[x][u], o[x][d], 0, 0, 0);
+            }
+        add_weights<CT>(pf, l);
+        if (odd) mark_nans<CT, DT>([&](int d) { return load_value(rows, d); }, seen, g, o);
         if (following.page >= 0) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) vr[d] = load_value(rows_next, d);
@@ -366,24 +410,8 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
         item = following;
         rows = rows_next;
     }
-    if (OWN_COLUMNS) {
-#pragma unroll
-        for (int x = 0; x < CT; ++x) {
-            const int y = first_col + 16 * x + col;
-            if (y >= columns) continue;
-            const int64_t r = row_of(y);
-            const float inv = l[x][0] == 0.f ? 0.f : pow2(unit) / l[x][0];
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                bf16x4 y;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] = (bf16_t)(o[x][d][i] * inv);
-                *reinterpret_cast<bf16x4*>(a.out + r * D + 16 * d + 4 * g) = y;
-            }
-        }
-        return;
-    }
-    // ---- join the waves, one column tile at a time: thread: column cc, four d's from dd on
+
+    // ---- join the waves, one column tile at a time: thread: column cc, four d's from d on
     extern __shared__ float shared[];  // so [W][16][D + 4], sm [W][16], sl [W][16]
     float *so = shared, *sm = so + W * 16 * (D + 4), *sl = sm + W * 16;
     constexpr int PER = D / 4;  // threads per column
@@ -401,7 +429,7 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
         for (int cc = threadIdx.x / PER; cc < 16; cc += 64 * W / PER) {
             const int d = 4 * (threadIdx.x % PER);
             const int y = first_col + 16 * x + cc;
-            if (y >= columns) break;
+            if (y >= cs.columns) break;
             float top = NEG_INF;
 #pragma unroll
             for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w * 16 + cc]);
@@ -414,8 +442,7 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
                 total += f * sl[w * 16 + cc];
                 v += *reinterpret_cast<const f32x4*>(so + (w * 16 + cc) * (D + 4) + d) * f;
             }
-            const int64_t r = row_of(y);
-            const int64_t rows = (int64_t)c.num_seqs * a.n * H * a.group;
+            const int64_t r = cs.row_of(y);
             if (a.splits == 1) {
                 const float inv = total == 0.f ? 0.f : 1.f / total;
                 bf16x4 b;
@@ -423,9 +450,175 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
                 for (int i = 0; i < 4; ++i) b[i] = (bf16_t)(v[i] * inv);
                 *reinterpret_cast<bf16x4*>(a.out + r * D + d) = b;
             } else {
-                *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)blockIdx.x * rows + r) * D + d) = v;
-                if (d == 0) a.part_ml[(int64_t)blockIdx.x * rows + r] = make_float2(top, total);
+                *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)blockIdx.x * a.rows + r) * D + d) = v;
+                if (d == 0) a.part_ml[(int64_t)blockIdx.x * a.rows + r] = make_float2(top, total);
             }
+        }
+    }
+}
+
+// Many columns (prompts): a workgroup of four waves has 128, each wave 32 of them, and all walk the same pages.  What bounds
+// it is vector instructions, and a fifth of those are conversions, so every page is converted once for the four waves: each
+// converts a quarter, into LDS, in the order in which the products' first operands are read (a lane's 16 bytes after
+// another's: no bank conflict).  Two buffers, one barrier per page; the next page's bytes are on their way meanwhile.
+constexpr int PROMPT_W = 4, PROMPT_CT = 2;
+// (D 64: 4 waves per SIMD, a few spilled registers included: 16 prompts of 4096 tokens 684 us; 3 waves 738.)
+constexpr int prompt_occupancy(int D) { return D == 64 ? 4 : 2; }
+template <int D>
+__global__ __launch_bounds__(64 * PROMPT_W) __attribute__((amdgpu_waves_per_eu(prompt_occupancy(D), prompt_occupancy(D))))
+void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
+    constexpr int CT = PROMPT_CT, W = PROMPT_W;
+    constexpr int KS = D / 64, DT = D / 16, OWN = DT / W;  // value tiles that a wave converts
+    constexpr int K_BYTES = ASRK_KV_PAGE * D * 2, BUF = 2 * K_BYTES;
+    extern __shared__ __attribute__((aligned(16))) char tiles[];  // [2][keys | values]
+    __shared__ int most_of[W];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const Columns probe(c, a, 0);
+    const int chunks = (probe.columns + 16 * CT * W - 1) / (16 * CT * W);
+    // The last rows of every prompt first: they see the most, and what is left for the end is short.
+    const int sets = c.num_seqs / a.beams, set = blockIdx.z % sets, chunk = chunks - 1 - blockIdx.z / sets;
+    const Columns cs(c, a, set);
+    const int first_col = (chunk * W + wave) * 16 * CT;
+    Pages work(c, a.beams, set, blockIdx.x, a.splits);
+    Queries<D, CT> qs;
+    qs.load(c, cs, first_col, col, g);
+    if (lane == 0) most_of[wave] = qs.most;
+    __syncthreads();
+    int most = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) most = most_of[w] > most ? most_of[w] : most;
+    const int pages = __builtin_amdgcn_readfirstlane((most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE);
+
+    f32x4 o[CT][DT], l[CT];
+    float m[CT];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+        m[t] = NEG_INF;
+        l[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    int unit = ASRK_KV_EXP_MIN, tile_unit = ASRK_KV_EXP_MIN;  // of o, and of the value tiles: the largest exponent so far
+
+    const char* layer = (const char*)c.kv + a.layer * c.num_pages * cs.H * (int64_t)(2 * ASRK_KV_PAGE * D);
+    const int* exps = (const int*)c.exps + a.layer * c.num_pages * cs.H;
+    // this lane's bytes of the wave's quarter: keys of tile `wave`, values of tiles wave * OWN ..
+    const uint32_t k_at = (16 * (col >> 2) + 4 * wave + (col & 3)) * D + 16 * g, v_at = col * ASRK_KV_PAGE + 16 * g;
+    u32x4 kr[KS], vr[OWN];
+    auto load_value = [&](__amdgpu_buffer_rsrc_t rows, int d) __attribute__((always_inline)) {
+        return __builtin_amdgcn_raw_buffer_load_b128(rows, v_at + 16 * d * ASRK_KV_PAGE, ASRK_KV_PAGE * D, 0);
+    };
+    auto load_page = [&](__amdgpu_buffer_rsrc_t rows) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kr[s] = __builtin_amdgcn_raw_buffer_load_b128(rows, k_at + 64 * s, 0, 0);
+#pragma unroll
+        for (int d = 0; d < OWN; ++d)
+            vr[d] = __builtin_amdgcn_raw_buffer_load_b128(rows, v_at + (wave * OWN + d) * (16 * ASRK_KV_PAGE), ASRK_KV_PAGE * D, 0);
+    };
+    Item item = work.next(pages);
+    int64_t at = (int64_t)(item.page < 0 ? 0 : item.page) * cs.H + cs.h;
+    __amdgpu_buffer_rsrc_t rows = page_rows(layer, at, D);
+    int e_next = 0;
+    if (item.page >= 0) {
+        e_next = exps[at];
+        load_page(rows);
+    }
+    char* buf = tiles;
+    while (item.page >= 0) {
+        const Item following = work.next(pages);
+        at = (int64_t)(following.page < 0 ? 0 : following.page) * cs.H + cs.h;
+        const __amdgpu_buffer_rsrc_t rows_next = page_rows(layer, at, D);
+        const int e = __builtin_amdgcn_readfirstlane(e_next);
+        if (following.page >= 0) e_next = exps[at];
+        const int ev = (int8_t)(e >> 8), up = ev > tile_unit ? ev : tile_unit;
+        tile_unit = up;
+        const bool odd = __builtin_expect((e >> 16) & 1, 0);
+        {
+            const float ks = pow2((int8_t)e), vs = pow2(ev - up);
+            if (a.beams > 1 || most < (item.p + 1) * ASRK_KV_PAGE) {  // the page may end within
+                KEEP_BRANCH();
+                const u32x4 mask = keep_before(tokens_held(c, set, a.beams, item.with, item.p), g);
+#pragma unroll
+                for (int d = 0; d < OWN; ++d) vr[d] &= mask;
+            }
+            if (odd) {
+                KEEP_BRANCH();
+#pragma unroll
+                for (int d = 0; d < OWN; ++d)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) vr[d][w] &= ~nan_bytes(vr[d][w]);
+            }
+            // fragment (tile, step): 64 lanes of 16 bytes
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                bf16x8* to = reinterpret_cast<bf16x8*>(buf) + (wave * 2 * KS + 2 * s) * 64 + lane;
+                to[0] = k8(kr[s][0], kr[s][1], ks);
+                to[64] = k8(kr[s][2], kr[s][3], ks);
+            }
+#pragma unroll
+            for (int d = 0; d < OWN; ++d) {
+                f16x8* to = reinterpret_cast<f16x8*>(buf + K_BYTES) + (wave * OWN + d) * 128 + lane;
+                to[0] = v8(vr[d][0], vr[d][1], vs);
+                to[64] = v8(vr[d][2], vr[d][3], vs);
+            }
+        }
+        __syncthreads();  // the other buffer was last read before the barrier in front of this one
+        if (following.page >= 0) load_page(rows_next);
+        int seen[CT];
+        bool whole;
+        if (qs.see(item.p, item.with, seen, whole)) {
+            const bf16x8* kt = reinterpret_cast<const bf16x8*>(buf) + lane;
+            const f16x8* vt = reinterpret_cast<const f16x8*>(buf + K_BYTES) + lane;
+            f32x4 sc[CT][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int x = 0; x < CT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < 2 * KS; ++s) {
+                    const bf16x8 k = kt[(t * 2 * KS + s) * 64];
+#pragma unroll
+                    for (int x = 0; x < CT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qs.q[x][s], sc[x][t], 0, 0, 0);
+                }
+            }
+            f16x8 pf[CT][2];
+            weigh<CT, DT>(sc, seen, whole, g, a.c, up, unit, m, l, o, pf);
+            unit = up;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const f16x8 v = vt[(d * 2 + u) * 64];
+#pragma unroll
+                    for (int x = 0; x < CT; ++x) o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[x][u], o[x][d], 0, 0, 0);
+                }
+            add_weights<CT>(pf, l);
+            if (odd) mark_nans<CT, DT>([&](int d) { return load_value(rows, d); }, seen, g, o);
+        }
+        buf = buf == tiles ? tiles + BUF : tiles;
+        item = following;
+        rows = rows_next;
+    }
+    const float u = pow2(unit);
+#pragma unroll
+    for (int x = 0; x < CT; ++x) {
+        const int y = first_col + 16 * x + col;
+        if (y >= cs.columns) continue;
+        const int64_t r = cs.row_of(y);
+        if (a.splits == 1) {
+            const float inv = l[x][0] == 0.f ? 0.f : u / l[x][0];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                bf16x4 b;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] = (bf16_t)(o[x][d][i] * inv);
+                *reinterpret_cast<bf16x4*>(a.out + r * D + 16 * d + 4 * g) = b;
+            }
+        } else {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)blockIdx.x * a.rows + r) * D + 16 * d + 4 * g) = o[x][d] * u;
+            if (g == 0) a.part_ml[(int64_t)blockIdx.x * a.rows + r] = make_float2(m[x], l[x][0]);
         }
     }
 }
@@ -460,10 +653,10 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __r
 
 struct Plan {
     int ct, waves, splits, chunks;
-    bool own;
+    bool prompt;
 };
 // By the capacity of the table, not by the lengths, which only the device knows.
-//  - 128 columns or more: four waves with columns of their own, each over all pages.
+//  - 128 columns or more: kv_prompt_kernel.
 //  - Fewer: the waves of a workgroup share them and deal the pages.  Up to 48 pages one workgroup does it all: a second
 //    launch to join splits costs 4 us, more than it saves (5 beams over 26 pages, 5 heads: 11.9 us, in 4 splits 15.8;
 //    64 times that: 19.6, in 2 splits 27.8).  Beyond, enough splits for 1024 workgroups, of two pages per wave at least
@@ -471,36 +664,40 @@ struct Plan {
 Plan plan_of(const asrk_kv_cache* c, int n, int q_heads, int beams) {
     const int64_t columns = (int64_t)beams * n * (q_heads / c->kv_heads);
     Plan p;
-    p.own = columns >= 128;
+    p.prompt = columns >= 128;
     p.ct = columns > 16 ? 2 : 1;
-    p.waves = p.own || p.ct == 2 ? 4 : 8;
-    const int per = 16 * p.ct * (p.own ? p.waves : 1);
+    p.waves = p.prompt || p.ct == 2 ? 4 : 8;
+    const int per = 16 * p.ct * (p.prompt ? p.waves : 1);
     p.chunks = (int)((columns + per - 1) / per);
     p.splits = 1;
-    if (!p.own && c->max_pages > 48) {
-        const int64_t groups = (int64_t)c->kv_heads * (c->num_seqs / beams) * p.chunks;
-        const int64_t want = (1024 + groups - 1) / groups, most = c->max_pages / (2 * p.waves);
+    const int64_t groups = (int64_t)c->kv_heads * (c->num_seqs / beams) * p.chunks;
+    const int64_t want = ((p.prompt ? 512 : 1024) + groups - 1) / groups, most = c->max_pages / (p.prompt ? 16 : 2 * p.waves);
+    if (c->max_pages > 48) {
         p.splits = (int)(want < most ? want : most);
         if (p.splits > 128) p.splits = 128;
     }
     return p;
 }
 
-template <int D, int CT, int W, bool OWN>
-int launch(const asrk_kv_cache* c, const AttnArgs& a, int sets, int chunks, hipStream_t st) {
-    constexpr int lds = OWN ? 0 : (W * 16 * (D + 4) + 2 * W * 16) * (int)sizeof(float);
-    if (lds > 65536) {
-        static std::atomic<uint64_t> done{0};
-        if (int rc = asrk_max_lds_once((const void*)kv_attention_kernel<D, CT, W, OWN>, lds, done)) return rc;
-    }
-    hipLaunchKernelGGL((kv_attention_kernel<D, CT, W, OWN>), dim3(a.splits, c->kv_heads, sets * chunks), dim3(64 * W), lds, st, *c, a);
+template <class K>
+int launch(K kernel, const asrk_kv_cache* c, const AttnArgs& a, int threads, int lds, int blocks, std::atomic<uint64_t>& done, hipStream_t st) {
+    if (lds > 65536)
+        if (int rc = asrk_max_lds_once((const void*)kernel, lds, done)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(a.splits, c->kv_heads, blocks), dim3(threads), lds, st, *c, a);
     return ASRK_OK;
+}
+template <int D, int CT, int W>
+int launch_shared(const asrk_kv_cache* c, const AttnArgs& a, int blocks, hipStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    return launch(kv_attention_kernel<D, CT, W>, c, a, 64 * W, (W * 16 * (D + 4) + 2 * W * 16) * (int)sizeof(float), blocks, done, st);
 }
 template <int D>
 int launch_for(const asrk_kv_cache* c, const AttnArgs& a, const Plan& p, int sets, hipStream_t st) {
-    if (p.own) return launch<D, 2, 4, true>(c, a, sets, p.chunks, st);
-    if (p.ct == 2) return launch<D, 2, 4, false>(c, a, sets, p.chunks, st);
-    return launch<D, 1, 8, false>(c, a, sets, p.chunks, st);
+    if (p.prompt) {
+        static std::atomic<uint64_t> done{0};
+        return launch(kv_prompt_kernel<D>, c, a, 64 * PROMPT_W, 4 * ASRK_KV_PAGE * D * 2, sets * p.chunks, done, st);
+    }
+    return p.ct == 2 ? launch_shared<D, 2, 4>(c, a, sets * p.chunks, st) : launch_shared<D, 1, 8>(c, a, sets * p.chunks, st);
 }
 
 int check_shape(const asrk_kv_cache* c, int n, int q_heads, int beams) {
@@ -542,6 +739,7 @@ extern "C" int asrk_kv_attention(const asrk_kv_cache* c, int layer, const void* 
     a.row_ld = row_ld;
     a.head_ld = head_ld;
     a.layer = layer;
+    a.rows = rows;
     a.n = n;
     a.group = q_heads / c->kv_heads;
     a.beams = num_beams;

@@ -40,7 +40,7 @@ def check_select(logits, scores, eos=None):
 
 @pytest.mark.parametrize("B,K,V,dtype,pad", [
     (1, 1, 2, "f32", 0), (2, 1, 3, "bf16", 0), (3, 2, 2, "f32", 1), (2, 16, 130, "f32", 0), (4, 8, 8192, "bf16", 0), (2, 3, 8193, "f32", 3),
-    (1, 5, 49157, "bf16", 59), (3, 5, 51865, "bf16", 0), (1, 16, 20001, "bf16", 0), (2, 7, 70001, "f32", 0), (130, 4, 97, "bf16", 0)])
+    (1, 5, 49157, "bf16", 59), (3, 5, 51865, "bf16", 0), (1, 16, 20001, "bf16", 0), (2, 7, 70001, "f32", 0), (130, 4, 97, "bf16", 0), (171, 12, 8197, "bf16", 0)])
 def test_select(B, K, V, dtype, pad):
     g = _gen(B * 1000 + V)
     x = (torch.randn((B * K, V + pad), generator=g, device="cuda") * 3).to(torch.bfloat16 if dtype == "bf16" else torch.float32)[:, :V]
@@ -334,7 +334,7 @@ def test_attend_several_tokens(dim, heads, group, n, margins):
     same_attention(c, o, q, scale=0.5, name="another scale")
 
 
-@pytest.mark.parametrize("dim,heads,group,beams,n", [(64, 5, 3, 5, 1), (128, 1, 4, 4, 1), (64, 1, 1, 32, 1), (64, 2, 2, 3, 3), (128, 2, 7, 5, 1), (64, 1, 8, 8, 2), (64, 1, 16, 4, 3)])
+@pytest.mark.parametrize("dim,heads,group,beams,n", [(64, 5, 3, 5, 1), (128, 1, 4, 4, 1), (64, 1, 1, 32, 1), (64, 2, 2, 3, 3), (128, 2, 7, 5, 1), (64, 1, 8, 8, 2), (64, 1, 16, 4, 3), (128, 1, 16, 5, 4)])
 def test_attend_beams(dim, heads, group, beams, n, margins):
     """Beams that share all pages but the last, some, or none; num_beams says which are worked on together and nothing else."""
     rng = np.random.default_rng(beams)
@@ -386,6 +386,17 @@ def test_attend_over_pages_of_very_different_scales():
         q = torch.from_numpy(rng.standard_normal((2, 64, 2, 64))).cuda().bfloat16()
         same_attention(c, o, q)
         same_attention(c, o, q[:, :1])
+
+
+@pytest.mark.parametrize("beams,n,group", [(1, 1, 2), (1, 8, 4), (1, 40, 4), (3, 1, 4), (2, 20, 4)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_splits_long_caches(dim, beams, n, group, margins):
+    """Over 48 pages the tokens are split over workgroups and joined, for few columns and for many."""
+    rng = np.random.default_rng(beams + n)
+    S = 2 * beams
+    c, o = filled(rng, S, 1, dim, [3300, 64 * 40][:1] * beams + [64 * 40] * beams, [n] * S, beams, np.array([3200, 64 * 39]))
+    q = torch.from_numpy(rng.standard_normal((S, n, group, dim))).cuda().bfloat16()
+    same_attention(c, o, q, beams=beams, margins=margins, name=f"3300 tokens, {beams} beams, {n} tokens, d {dim}")
 
 
 def test_attend_takes_any_strides():

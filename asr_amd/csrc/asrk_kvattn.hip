@@ -82,7 +82,7 @@ struct Columns {
     const AttnArgs& a;
     int set, h, H, per_seq, columns;
     __device__ __forceinline__ Columns(const asrk_kv_cache& c, const AttnArgs& args, int set_)
-        : a(args), set(set_), h(blockIdx.y), H(c.kv_heads), per_seq(args.n * args.group), columns(args.beams * per_seq) {}
+        : a(args), set(set_), h(blockIdx.x / args.splits % c.kv_heads), H(c.kv_heads), per_seq(args.n * args.group), columns(args.beams * per_seq) {}
     __device__ __forceinline__ void split(int y, int& b, int& i, int& j) const {
         b = a.beams == 1 ? 0 : (int)((unsigned)y / (unsigned)per_seq);
         const unsigned in = (unsigned)(y - b * per_seq);
@@ -301,11 +301,11 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     constexpr int DT = D / 16;   // tiles of 16 d
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int sets = c.num_seqs / a.beams, set = blockIdx.z % sets;
+    const int part = blockIdx.x % a.splits, block = blockIdx.x / a.splits / c.kv_heads, sets = c.num_seqs / a.beams, set = block % sets;
     const Columns cs(c, a, set);
-    const int first_col = blockIdx.z / sets * 16 * CT;
+    const int first_col = block / sets * 16 * CT;
     // The pages of a wave: by its number alone, so that their numbers are on the way before the lengths are known.
-    Pages work(c, a.beams, set, blockIdx.x * W + wave, a.splits * W);
+    Pages work(c, a.beams, set, part * W + wave, a.splits * W);
     Queries<D, CT> qs;
     qs.load(c, cs, first_col, col, g);
     const int pages = (qs.most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
@@ -450,8 +450,8 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
                 for (int i = 0; i < 4; ++i) b[i] = (bf16_t)(v[i] * inv);
                 *reinterpret_cast<bf16x4*>(a.out + r * D + d) = b;
             } else {
-                *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)blockIdx.x * a.rows + r) * D + d) = v;
-                if (d == 0) a.part_ml[(int64_t)blockIdx.x * a.rows + r] = make_float2(top, total);
+                *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)part * a.rows + r) * D + d) = v;
+                if (d == 0) a.part_ml[(int64_t)part * a.rows + r] = make_float2(top, total);
             }
         }
     }
@@ -477,10 +477,10 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
     const Columns probe(c, a, 0);
     const int chunks = (probe.columns + 16 * CT * W - 1) / (16 * CT * W);
     // The last rows of every prompt first: they see the most, and what is left for the end is short.
-    const int sets = c.num_seqs / a.beams, set = blockIdx.z % sets, chunk = chunks - 1 - blockIdx.z / sets;
+    const int part = blockIdx.x % a.splits, block = blockIdx.x / a.splits / c.kv_heads, sets = c.num_seqs / a.beams, set = block % sets, chunk = chunks - 1 - block / sets;
     const Columns cs(c, a, set);
     const int first_col = (chunk * W + wave) * 16 * CT;
-    Pages work(c, a.beams, set, blockIdx.x, a.splits);
+    Pages work(c, a.beams, set, part, a.splits);
     Queries<D, CT> qs;
     qs.load(c, cs, first_col, col, g);
     if (lane == 0) most_of[wave] = qs.most;
@@ -617,8 +617,8 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
             }
         } else {
 #pragma unroll
-            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)blockIdx.x * a.rows + r) * D + 16 * d + 4 * g) = o[x][d] * u;
-            if (g == 0) a.part_ml[(int64_t)blockIdx.x * a.rows + r] = make_float2(m[x], l[x][0]);
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)part * a.rows + r) * D + 16 * d + 4 * g) = o[x][d] * u;
+            if (g == 0) a.part_ml[(int64_t)part * a.rows + r] = make_float2(m[x], l[x][0]);
         }
     }
 }
@@ -681,9 +681,9 @@ Plan plan_of(const asrk_kv_cache* c, int n, int q_heads, int beams) {
 
 template <class K>
 int launch(K kernel, const asrk_kv_cache* c, const AttnArgs& a, int threads, int lds, int blocks, std::atomic<uint64_t>& done, hipStream_t st) {
-    if (lds > 65536)
+    if (lds > 60000)  // beside what the kernel declares itself, 64 KiB need asking for
         if (int rc = asrk_max_lds_once((const void*)kernel, lds, done)) return rc;
-    hipLaunchKernelGGL(kernel, dim3(a.splits, c->kv_heads, blocks), dim3(threads), lds, st, *c, a);
+    hipLaunchKernelGGL(kernel, dim3(blocks * c->kv_heads * a.splits), dim3(threads), lds, st, *c, a);
     return ASRK_OK;
 }
 template <int D, int CT, int W>
@@ -719,11 +719,11 @@ extern "C" int asrk_kv_attention(const asrk_kv_cache* c, int layer, const void* 
                                  int q_heads, int num_beams, float scale, void* out, void* ws, size_t ws_bytes, void* stream) {
     if (int rc = check_shape(c, n, q_heads, num_beams)) return rc;
     if (!q || !out) return ASRK_ERR_NULL;
-    if (layer < 0 || layer >= c->num_layers || seq_ld < 0 || row_ld < 0 || head_ld < 0 || !(scale > 0.f)) return ASRK_ERR_SHAPE;
+    if (layer < 0 || layer >= c->num_layers || seq_ld < 0 || row_ld < 0 || head_ld < 0 || !(scale > 0.f && scale < 1e30f)) return ASRK_ERR_SHAPE;
     if (((uintptr_t)q & 15) || ((uintptr_t)out & 15) || seq_ld % 8 || row_ld % 8 || head_ld % 8) return ASRK_ERR_ALIGN;
     const Plan p = plan_of(c, n, q_heads, num_beams);
     const int sets = c->num_seqs / num_beams;
-    if ((int64_t)sets * p.chunks > 65535) return ASRK_ERR_SHAPE;
+    if ((int64_t)sets * p.chunks * c->kv_heads * p.splits > 0x7fffffff) return ASRK_ERR_SHAPE;
     const int64_t rows = (int64_t)c->num_seqs * n * q_heads;
     AttnArgs a{};
     if (p.splits > 1) {

@@ -162,6 +162,7 @@ class PagedKVCache:
             cache.extend(1)
             ... cache.write(k, v, layer=l); o = cache.attend(q, layer=l, num_beams=K) ...
 
+    ``max_len`` is rounded up to whole pages; ``num_pages`` is room for all sequences at that length unless it is given.
     The cache and its views belong to one stream at a time.  Its tensors (``kv``, ``exps``, ``table``, ``lens``, ``starts``,
     ``refs``: the layout is that of ``asrk_kv_cache`` in include/asrk.h) may be read, and overwritten in place; they are
     never replaced, so a captured step stays valid.  Calls that cannot be carried out on the device (no free page, a
@@ -280,7 +281,8 @@ class PagedKVCache:
 
     def write(self, k: torch.Tensor, v: torch.Tensor, layer: int = 0) -> None:
         """The new tokens' keys and values of one layer: ``k``, ``v`` [num_seqs, n, kv_heads, head_dim] (float32 or bfloat16, any
-        strides).  Row i of sequence s is its token ``starts[s] + i``; rows behind ``lens[s]`` are not looked at."""
+        strides).  Row i of sequence s is its token ``starts[s] + i``; rows behind ``lens[s]`` are not looked at, and new tokens
+        that no row is given for are not written."""
         shape = (self.num_seqs, self.kv_heads, self.head_dim)
         if k.dim() != 4 or k.shape != v.shape or (k.shape[0], *k.shape[2:]) != shape:
             raise ValueError(f"k and v must be [{shape[0]}, n, {shape[1]}, {shape[2]}], got {list(k.shape)} and {list(v.shape)}")
@@ -336,8 +338,8 @@ class PagedKVCache:
         if not 1 <= num_beams <= 32 or self.num_seqs % num_beams:
             raise ValueError(f"{self.num_seqs} sequences are not groups of {num_beams} (at most 32)")
         scale = self.head_dim ** -0.5 if scale is None else float(scale)
-        if not 0 < scale < float("inf"):
-            raise ValueError(f"scale must be positive and finite, got {scale}")
+        if not 1e-30 < scale < 1e30:
+            raise ValueError(f"scale must be positive, got {scale}")
         self._mine("attend", q)
         layer = self._layer(layer)
         out = q.new_empty(q.shape)

@@ -164,6 +164,8 @@ def test_c_abi_refusals():
         return lib.asrk_kv_attention(c, layer, q, *lds, n, heads, beams, 0.125, out, ws, ws_bytes, None)
 
     assert attend(q=None) == NULL and attend(out=None) == NULL and attend(layer=2) == SHAPE and attend(n=0) == SHAPE
+    assert lib.asrk_kv_attention(c, 0, p, 256, 128, 64, 1, 4, 1, 0.0, p, p, 1 << 30, None) == SHAPE
+    assert lib.asrk_kv_attention(c, 0, p, 256, 128, 64, 1, 4, 1, float("nan"), p, p, 1 << 30, None) == SHAPE
     assert attend(heads=3) == SHAPE and attend(heads=0) == SHAPE and attend(beams=3) == SHAPE and attend(beams=0) == SHAPE
     assert attend(lds=(256, 4, 64)) == ALIGN and attend(out=p + 8) == ALIGN
     big = _cache_struct(max_pages=100)

@@ -250,6 +250,30 @@ def test_pages_over_a_random_life(seed):
         same_tokens(c, o, 0, 330)
 
 
+def test_pages_of_thousands_of_sequences():
+    """More sequences than threads in the workgroup that hands out pages, and more pages than it looks at in one go."""
+    rng = np.random.default_rng(77)
+    B, K = 700, 3
+    c, o = both(B * K, 192, 1, 64, pages=20000)
+    lead = c.leaders(K)
+    for n in (rng.integers(0, 100, B), rng.integers(0, 3, B)):
+        lead.extend(torch.from_numpy(n).cuda())
+        o.extend(n, K)
+        same_pages(c, o)
+    for _ in range(3):
+        par = rng.integers(0, K, (B, K)) * (rng.random((B, 1)) < 0.7)
+        par = np.where(rng.random((B, K)) < 0.1, -1, par)
+        c.reorder(torch.from_numpy(par).cuda())
+        o.reorder(par)
+        n = rng.integers(0, 30, B * K)
+        c.extend(torch.from_numpy(n).cuda())
+        o.extend(n)
+        same_pages(c, o)
+        assert int(c.compact()) == o.compact()
+        same_pages(c, o)
+    assert o.status in (0, 2)
+
+
 def test_what_does_not_fit_adds_nothing_and_is_reported():
     from asr_amd import _lib
 
@@ -399,6 +423,23 @@ def test_attend_splits_long_caches(dim, beams, n, group, margins):
     same_attention(c, o, q, beams=beams, margins=margins, name=f"3300 tokens, {beams} beams, {n} tokens, d {dim}")
 
 
+def test_attend_over_many_sequences():
+    """More workgroups than a grid's second and third dimensions hold."""
+    S, n, group = 9000, 100, 16
+    c, o = both(S, 110, 1, 64)
+    g = _gen(91)
+    for rows in (7, n):
+        c.extend(rows)
+        o.extend(rows)
+        k, v = (torch.randn((S, rows, 1, 64), generator=g, device="cuda").bfloat16() for _ in range(2))
+        c.write(k, v)
+        o.write(k[::3000].double().cpu().numpy(), v[::3000].double().cpu().numpy(), every=3000)
+    q = torch.randn((S, n, group, 64), generator=g, device="cuda").bfloat16()
+    got = c.attend(q)[::3000]
+    assert torch.equal(got, c.leaders(3000).attend(q[::3000]))
+    same_attention(c, o, q[::3000, :, :2], every=3000)
+
+
 def test_attend_takes_any_strides():
     rng = np.random.default_rng(10)
     c, o = filled(rng, 3, 2, 64, [70, 3, 100], [2, 2, 2], layers=2)
@@ -448,7 +489,7 @@ def test_refusals():
         with pytest.raises(ValueError):
             c.write(k, v)
     for q, kw in ((ok[:3], {}), (ok.float(), {}), (ok[:, :, :1], {}), (ok[..., :32], {}), (ok, dict(num_beams=3)), (ok, dict(num_beams=0)), (ok, dict(layer=2)),
-                  (ok, dict(layer=-1)), (ok[:, :, :0], {})):
+                  (ok, dict(layer=-1)), (ok[:, :, :0], {}), (ok, dict(scale=0.0)), (ok, dict(scale=-1.0)), (ok, dict(scale=math.nan)), (ok, dict(scale=math.inf))):
         with pytest.raises(ValueError):
             c.attend(q, **kw)
     with pytest.raises(ValueError):

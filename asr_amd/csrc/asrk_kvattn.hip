@@ -34,7 +34,7 @@ struct AttnArgs {
     float* part_o;   // [splits][S n Hq][D]
     float2* part_ml; // [splits][S n Hq]
     int64_t seq_ld, row_ld, head_ld, layer, rows;  // rows: S n Hq
-    int n, group, beams, splits;  // new tokens, query heads per key/value head
+    int n, group, beams, splits, chunks, sets;  // new tokens, query heads per key/value head, ..., groups of beams
     float c;
 };
 
@@ -97,7 +97,7 @@ struct Columns {
 };
 
 // What a lane holds of its CT columns: q as the second operand (16 consecutive d's per pair of steps), the beam, the number
-// of tokens seen; the largest such number of the wave.
+// of tokens seen; the largest such number of the lane.
 template <int D, int CT>
 struct Queries {
     bf16x8 q[CT][D / 32];
@@ -130,7 +130,6 @@ struct Queries {
                 }
             }
         }
-        most = __builtin_amdgcn_readfirstlane(wave_imax(most));
     }
     // Of page p, for the beams `with`: tokens seen by each column; whether all see all of it, and whether any sees any.
     __device__ __forceinline__ bool see(int p, uint64_t with, int* seen, bool& whole) const {
@@ -196,14 +195,6 @@ __device__ __forceinline__ u32x4 keep_before(int last, int g) {
     }
     return mask;
 }
-// Tokens that the longest of the beams `with` has of page p.
-__device__ __forceinline__ int tokens_held(const asrk_kv_cache& c, int set, int beams, uint64_t with, int p) {
-    const int lane = threadIdx.x & 63;
-    const int len = lane < beams && ((with >> lane) & 1) ? c.lens[((int64_t)set * beams + lane) * c.seq_stride] : 0;
-    const int held = __builtin_amdgcn_readfirstlane(wave_imax(len)) - p * ASRK_KV_PAGE;
-    return held < 0 ? 0 : (held > ASRK_KV_PAGE ? ASRK_KV_PAGE : held);
-}
-
 // Scores of one page to weights.  The reference follows the maximum only when that has grown by more than 2^8: up to there
 // the weights stay within f16, at the same relative precision, and o and the sum need no rescaling.
 template <int CT, int DT>
@@ -301,14 +292,14 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     constexpr int DT = D / 16;   // tiles of 16 d
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int part = blockIdx.x % a.splits, block = blockIdx.x / a.splits / c.kv_heads, sets = c.num_seqs / a.beams, set = block % sets;
+    const int part = blockIdx.x % a.splits, block = blockIdx.x / a.splits / c.kv_heads, set = block % a.sets;
     const Columns cs(c, a, set);
-    const int first_col = block / sets * 16 * CT;
+    const int first_col = block / a.sets * 16 * CT;
     // The pages of a wave: by its number alone, so that their numbers are on the way before the lengths are known.
     Pages work(c, a.beams, set, part * W + wave, a.splits * W);
     Queries<D, CT> qs;
     qs.load(c, cs, first_col, col, g);
-    const int pages = (qs.most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
+    const int pages = (__builtin_amdgcn_readfirstlane(wave_imax(qs.most)) + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
 
     f32x4 o[CT][DT], l[CT];
     float m[CT];
@@ -471,24 +462,43 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
     constexpr int KS = D / 64, DT = D / 16, OWN = DT / W;  // value tiles that a wave converts
     constexpr int K_BYTES = ASRK_KV_PAGE * D * 2, BUF = 2 * K_BYTES;
     extern __shared__ __attribute__((aligned(16))) char tiles[];  // [2][keys | values]
-    __shared__ int most_of[W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const Columns probe(c, a, 0);
-    const int chunks = (probe.columns + 16 * CT * W - 1) / (16 * CT * W);
     // The last rows of every prompt first: they see the most, and what is left for the end is short.
-    const int part = blockIdx.x % a.splits, block = blockIdx.x / a.splits / c.kv_heads, sets = c.num_seqs / a.beams, set = block % sets, chunk = chunks - 1 - block / sets;
+    const int part = blockIdx.x % a.splits, block = blockIdx.x / a.splits / c.kv_heads, set = block % a.sets, chunk = a.chunks - 1 - block / a.sets;
     const Columns cs(c, a, set);
     const int first_col = (chunk * W + wave) * 16 * CT;
     Pages work(c, a.beams, set, part, a.splits);
+    // Tokens of each beam (lane), and how many of them any column of the workgroup sees: of one sequence those up to its last
+    // row's own, of several at most all.
+    const int64_t seq = (int64_t)set * a.beams;
+    const int held_by = lane < a.beams ? c.lens[(seq + lane) * c.seq_stride] : 0;
+    int most;
+    if (a.beams == 1) {
+        const int start = c.starts[seq * c.seq_stride], fresh = __builtin_amdgcn_readfirstlane(held_by) - start;
+        const int x0 = chunk * W * 16 * CT, x1 = x0 + W * 16 * CT < cs.columns ? x0 + W * 16 * CT : cs.columns;
+        const int i0 = (int)((unsigned)x0 / (unsigned)a.group), i1 = (int)((unsigned)(x1 - 1) / (unsigned)a.group) + 1;
+        most = i0 >= fresh ? 0 : start + (i1 < fresh ? i1 : fresh);
+    } else {
+        most = __builtin_amdgcn_readfirstlane(wave_imax(held_by));
+    }
+    int pages = (most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
+    pages = pages < c.max_pages ? pages : c.max_pages;
+    if (pages <= 0) {  // nothing to see: the rows are zero
+        if (a.splits == 1) {
+#pragma unroll
+            for (int x = 0; x < CT; ++x) {
+                const int y = first_col + 16 * x + col;
+                if (y >= cs.columns) continue;
+                bf16_t* p = a.out + cs.row_of(y) * D + 4 * g;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) *reinterpret_cast<u32x2*>(p + 16 * d) = u32x2{0u, 0u};
+            }
+            return;
+        }
+    }
     Queries<D, CT> qs;
     qs.load(c, cs, first_col, col, g);
-    if (lane == 0) most_of[wave] = qs.most;
-    __syncthreads();
-    int most = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) most = most_of[w] > most ? most_of[w] : most;
-    const int pages = __builtin_amdgcn_readfirstlane((most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE);
 
     f32x4 o[CT][DT], l[CT];
     float m[CT];
@@ -536,9 +546,11 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
         const bool odd = __builtin_expect((e >> 16) & 1, 0);
         {
             const float ks = pow2((int8_t)e), vs = pow2(ev - up);
-            if (a.beams > 1 || most < (item.p + 1) * ASRK_KV_PAGE) {  // the page may end within
+            const int held = (a.beams == 1 ? __builtin_amdgcn_readfirstlane(held_by)
+                                           : __builtin_amdgcn_readfirstlane(wave_imax((item.with >> lane) & 1 ? held_by : 0))) - item.p * ASRK_KV_PAGE;
+            if (held < ASRK_KV_PAGE) {  // the sequence ends within the page
                 KEEP_BRANCH();
-                const u32x4 mask = keep_before(tokens_held(c, set, a.beams, item.with, item.p), g);
+                const u32x4 mask = keep_before(held, g);
 #pragma unroll
                 for (int d = 0; d < OWN; ++d) vr[d] &= mask;
             }
@@ -744,6 +756,8 @@ extern "C" int asrk_kv_attention(const asrk_kv_cache* c, int layer, const void* 
     a.group = q_heads / c->kv_heads;
     a.beams = num_beams;
     a.splits = p.splits;
+    a.chunks = p.chunks;
+    a.sets = sets;
     a.c = scale * 1.4426950408889634f;
     hipStream_t st = (hipStream_t)stream;
     if (int rc = c->head_dim == 64 ? launch_for<64>(c, a, p, sets, st) : launch_for<128>(c, a, p, sets, st)) return rc;

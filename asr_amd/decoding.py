@@ -108,8 +108,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, eos_token_id: Option
     scores = scores.contiguous()
     if ld < V:  # a single row, or rows that overlap
         logits, ld = logits.contiguous(), V
-    out = (scores.new_empty((B, K)), *scores.new_empty((2, B, K), dtype=torch.int64).unbind(0),
-           scores.new_empty((B, 2 * K)), *scores.new_empty((2, B, 2 * K), dtype=torch.int64).unbind(0))
+    # six tensors in one allocation (an as_strided is 0.8 us, an allocation 1.4): 6 B K integers, then 3 B K floats
+    ints, m = scores.new_empty((8 * B * K,), dtype=torch.int64), B * K
+    floats = ints.view(torch.float32)
+    one, two, ones, twos = (B, K), (B, 2 * K), (K, 1), (2 * K, 1)
+    out = (floats.as_strided(one, ones, 12 * m), ints.as_strided(one, ones, 0), ints.as_strided(one, ones, m),
+           floats.as_strided(two, twos, 13 * m), ints.as_strided(two, twos, 2 * m), ints.as_strided(two, twos, 4 * m))
     if B:
         need = _select_workspace(B, K, V)
         ws = scores.new_empty((need,), dtype=torch.uint8)

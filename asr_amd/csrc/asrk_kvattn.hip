@@ -197,8 +197,11 @@ __device__ __forceinline__ u32x4 keep_before(int last, int g) {
     }
     return mask;
 }
-// Scores of one page to weights.  The reference follows the maximum only when that has grown by more than 2^8: up to there
-// the weights stay within f16, at the same relative precision, and o and the sum need no rescaling.
+// Scores of one page to weights, 2^HEAD times what they are to the reference: f16's range is spent on the small ones.  A
+// weight of 2^-27 of the largest still has all 11 bits, and below that it is held to 2^-38 of the largest.  The reference
+// follows the maximum only when that has grown by more than 2^SLACK: up to there nothing overflows (2^15) and o and the sum
+// need no rescaling.
+constexpr float HEAD = 13.f, SLACK = 2.f;
 template <int CT, int DT>
 __device__ __forceinline__ void weigh(f32x4 (*sc)[4], const int* seen, bool whole, int g, float scale, int up, int unit, float* m, f32x4* l,
                                       f32x4 (*o)[DT], f16x8 (*pf)[2]) {
@@ -219,9 +222,9 @@ __device__ __forceinline__ void weigh(f32x4 (*sc)[4], const int* seen, bool whol
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[x][t][i]);
         const float now = groups_max(top) * scale;  // scale > 0
-        if (__any(now > m[x] + 8.f) || up != unit) {
+        if (__any(now > m[x] + SLACK) || up != unit) {
             KEEP_BRANCH();
-            const float to = now > m[x] + 8.f ? now : m[x];  // by the column alone: its bits do not depend on its neighbours
+            const float to = now > m[x] + SLACK ? now : m[x];  // by the column alone: its bits do not depend on its neighbours
             const float back = to > NEG_INF ? __builtin_amdgcn_exp2f(m[x] - to) : 0.f;
             m[x] = to;
 #pragma unroll
@@ -229,7 +232,7 @@ __device__ __forceinline__ void weigh(f32x4 (*sc)[4], const int* seen, bool whol
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[x][d] *= back * shrink;
         }
-        const float ref = m[x] > NEG_INF ? m[x] : 0.f;  // nothing seen yet: every weight is 0
+        const float ref = m[x] > NEG_INF ? m[x] - HEAD : 0.f;  // nothing seen yet: every weight is 0
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll

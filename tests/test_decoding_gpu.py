@@ -21,6 +21,12 @@ def _gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
 
+def PagedKVCache_(*args, **kw):
+    from asr_amd.decoding import PagedKVCache
+
+    return PagedKVCache(*args, **kw)
+
+
 # ---- selection
 
 
@@ -438,6 +444,30 @@ def test_attend_over_many_sequences():
     got = c.attend(q)[::3000]
     assert torch.equal(got, c.leaders(3000).attend(q[::3000]))
     same_attention(c, o, q[::3000, :, :2], every=3000)
+
+
+@pytest.mark.parametrize("n", [1, 130])
+@pytest.mark.parametrize("low", [8.0, 14.2, 17.3, 20.0])
+def test_attend_adds_up_many_small_weights(n, low):
+    """One token that outweighs each of 20000 others by 2**(low * 1.44): what they add up to is the result, to its own size (and
+    half a step of 2**-37, times the largest weight, for each of them: weights below 2**-27 of the largest are subnormal)."""
+    c = PagedKVCache_(1, 20300, 1, 64)
+    k, v = (torch.zeros((1, 20000, 1, 64), device="cuda") for _ in range(2))
+    k[:, 0, :, 0] = 2.0 ** round(math.log2(low))
+    v[:, 1:] = 1.0
+    c.extend(20000)
+    c.write(k, v)
+    c.extend(n)
+    c.write(torch.zeros((1, n, 1, 64), device="cuda"), torch.ones((1, n, 1, 64), device="cuda"))
+    q = torch.zeros((1, n, 1, 64), device="cuda", dtype=torch.bfloat16)
+    top = float(torch.tensor(low * 8 / 2.0 ** round(math.log2(low))).bfloat16())  # q.k / 8 is about low
+    q[..., 0] = top
+    s = top * 2.0 ** round(math.log2(low)) / 8
+    got = c.attend(q).double().cpu().numpy()
+    others = 20000 + np.arange(n).reshape(1, n, 1, 1)  # tokens of weight exp(-s) and value 1
+    want = others * math.exp(-s) / (1 + others * math.exp(-s))
+    over = np.abs(got - want) / (want * (2.0 ** -8 + 2.0 ** -10) + others * 2.0 ** -38)
+    assert over.max() <= 1, over.max()
 
 
 def test_attend_takes_any_strides():

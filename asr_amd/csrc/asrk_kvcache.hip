@@ -232,22 +232,19 @@ __global__ __launch_bounds__(64) void kv_reorder_kernel(asrk_kv_cache c, const i
     }
     if (blockIdx.x == 0) {  // one wave: all lengths are read before any is written
         const int k = threadIdx.x;
-        int len = 0, start = 0;
+        int len = 0;
         if (k < K) {
             int64_t p = par[k];
             if (p < -1 || p >= K) {
                 atomicOr(&c.status[0], ASRK_KV_BAD_PARENT);
                 p = k;
             }
-            if (p >= 0) {
-                len = c.lens[first + p * c.seq_stride];
-                start = c.starts[first + p * c.seq_stride];
-            }
+            if (p >= 0) len = c.lens[first + p * c.seq_stride];
         }
         __syncthreads();
         if (k < K) {
             c.lens[first + (int64_t)k * c.seq_stride] = len;
-            c.starts[first + (int64_t)k * c.seq_stride] = start;
+            c.starts[first + (int64_t)k * c.seq_stride] = len;  // no token is new: a write before the next extend could meet a shared page
         }
     }
 }

@@ -235,7 +235,8 @@ class PagedKVCache:
 
     def reorder(self, parents: torch.Tensor) -> None:
         """Beam k of utterance b goes on as a copy of its beam ``parents[b, k]``; -1 empties it and gives its pages back.
-        int64 [B, K], B * K == num_seqs, K <= 32.  Only page numbers move."""
+        int64 [B, K], B * K == num_seqs, K <= 32.  Only page numbers move.  No token of any sequence is new afterwards: ``extend``
+        comes next."""
         parents = _check_parents("reorder", parents)
         if parents.numel() != self.num_seqs or parents.shape[1] > 32:
             raise ValueError(f"parents must be [B, K] with B * K == {self.num_seqs} and K <= 32, got {list(parents.shape)}")

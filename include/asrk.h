@@ -287,8 +287,8 @@ size_t asrk_kv_scratch_bytes(int num_pages, int num_slots);
  * max_pages * 64, only starts = lens is done and `status` says why. */
 int asrk_kv_extend(const asrk_kv_cache* c, const int32_t* n_each, int n_all, void* stream);
 
-/* Sequence b K + k becomes what b K + parents[b][k] was, -1: empty (parents dev int64 [num_seqs / K][K], K <= 32).  No
- * page is copied.  Any other value leaves the sequence as it was and sets ASRK_KV_BAD_PARENT. */
+/* Sequence b K + k becomes what b K + parents[b][k] was, -1: empty (parents dev int64 [num_seqs / K][K], K <= 32), with no
+ * new tokens (starts = lens).  No page is copied.  Any other value leaves the sequence as it was and sets ASRK_KV_BAD_PARENT. */
 int asrk_kv_reorder(const asrk_kv_cache* c, const int64_t* parents, int K, void* stream);
 
 /* Moves pages so that those in use are 0 .. status[1] - 1.  seq_stride must be 1. */

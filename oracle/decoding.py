@@ -103,16 +103,17 @@ class Cache:
     def reorder(self, parents):
         parents = np.asarray(parents)
         B, K = parents.shape
-        table, lens, starts = self.table.copy(), self.lens.copy(), self.starts.copy()
+        table, lens = self.table.copy(), self.lens.copy()
         for b in range(B):
             for k in range(K):
                 p, s = parents[b, k], b * K + k
                 if p == -1:
-                    self.table[s], self.lens[s], self.starts[s] = -1, 0, 0
+                    self.table[s], self.lens[s] = -1, 0
                 elif 0 <= p < K:
-                    self.table[s], self.lens[s], self.starts[s] = table[b * K + p], lens[b * K + p], starts[b * K + p]
+                    self.table[s], self.lens[s] = table[b * K + p], lens[b * K + p]
                 else:
                     self.status |= 8
+        self.starts = self.lens.copy()
 
     def compact(self):
         used = np.flatnonzero(self.refs > 0)

@@ -381,6 +381,13 @@ def test_attend_beams(dim, heads, group, beams, n, margins):
     par = rng.integers(0, beams, (3, beams))  # pages shared in no order
     c.reorder(torch.from_numpy(par).cuda())
     o.reorder(par)
+    assert int((c.attend(q, num_beams=beams) != 0).sum()) == 0  # nothing is new
+    new = np.minimum(n, rng.integers(0, 2 * n + 1, S))
+    c.extend(torch.from_numpy(new).cuda())
+    o.extend(new)
+    k, v = (torch.from_numpy(rng.standard_normal((S, n, heads, dim))).float().cuda() for _ in range(2))
+    c.write(k, v)
+    o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
     same_attention(c, o, q, beams=beams, name="reordered")
 
 
@@ -468,6 +475,25 @@ def test_attend_adds_up_many_small_weights(n, low):
     want = others * math.exp(-s) / (1 + others * math.exp(-s))
     over = np.abs(got - want) / (want * (2.0 ** -8 + 2.0 ** -10) + others * 2.0 ** -38)
     assert over.max() <= 1, over.max()
+
+
+def test_a_write_after_reorder_waits_for_extend():
+    """Beams that have just come to share a page do not write into it."""
+    rng = np.random.default_rng(5)
+    c, o = filled(rng, 3, 1, 64, [70, 70, 70], [1, 1, 1], 3, np.array([60]))
+    par = np.array([[1, 1, 1]])
+    c.reorder(torch.from_numpy(par).cuda())
+    o.reorder(par)
+    before = c.kv.clone(), c.exps.clone()
+    k, v = (torch.randn((3, 1, 1, 64), device="cuda") * 100 for _ in range(2))
+    c.write(k, v)
+    assert torch.equal(c.kv, before[0]) and torch.equal(c.exps, before[1])
+    c.extend(1)
+    o.extend(1)
+    c.write(k, v)
+    o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+    same_pages(c, o)
+    same_tokens(c, o, 0, 80)
 
 
 def test_attend_takes_any_strides():

@@ -11,9 +11,9 @@
 //   O^T = V^T P^T (16x16x32 f16)   the lane's 16 weights are the second operand as they are, and 16 consecutive tokens of
 //                                  one d are 16 bytes of the value page
 // Columns are the rows of q that share a key/value head: beams x new tokens x query heads per key/value head.
-// Keys become bf16 with their scale applied (exact); values become f16 in units of 2^E, E the largest exponent so far:
-// exact up to a ratio of 2^15 between pages, below that to 2^-25 of the largest value.  Weights are rounded to f16, 2^-11
-// relative, 8 times finer than bf16 would be and well under the 2^-8 of the bf16 result.  Everything else is fp32.
+// Keys become bf16 with their scale applied (exact); values become f16 in a unit that follows the pages' scales (exact, for
+// pages up to 2^90 apart).  Weights are rounded to f16, 2^-11 relative, 8 times finer than bf16 would be and well under the
+// 2^-8 of the bf16 result.  Everything else is fp32.
 // Measured: 1.2 GB of cache (48 sequences, 8 heads of 128) 204 us = 5.9 TB/s; 64 x 5 beams over 1641 tokens that share their
 // prompts (64 MB) 20 us; one utterance 12 us, latency.
 #include "asrk_kvcache.h"
@@ -197,6 +197,20 @@ __device__ __forceinline__ u32x4 keep_before(int last, int g) {
     }
     return mask;
 }
+// Values are multiplied, and o is held, in units of 2^now.  An e4m3 value times 2^-15 .. 2^7 is exact in f16, so the unit
+// stays while a page's exponent lies in that window, and else follows it up or down -- down at most 2^75 below the largest
+// exponent so far, where o cannot leave fp32's range yet.  (A unit that only rises would round the values of a beam, or of a
+// page, by those of another that happens to come before.)
+struct Unit {
+    int now = ASRK_KV_EXP_MIN, top = ASRK_KV_EXP_MIN;
+    __device__ __forceinline__ int follow(int ev) {
+        top = ev > top ? ev : top;
+        const int d = ev - now;
+        if (d > 7 || d < -15) now = ev > top - 75 ? ev : top - 75;
+        return now;
+    }
+};
+
 // Scores of one page to weights, 2^HEAD times what they are to the reference: f16's range is spent on the small ones.  A
 // weight of 2^-27 of the largest still has all 11 bits, and below that it is held to 2^-38 of the largest.  The reference
 // follows the maximum only when that has grown by more than 2^SLACK: up to there nothing overflows (2^15) and o and the sum
@@ -315,7 +329,8 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    int unit = ASRK_KV_EXP_MIN;  // o is in units of 2^unit
+    Unit unit;
+    int held_unit = unit.now;  // of o
 
     const char* layer = (const char*)c.kv + a.layer * c.num_pages * cs.H * (int64_t)(2 * ASRK_KV_PAGE * D);
     const int* exps = (const int*)c.exps + a.layer * c.num_pages * cs.H;
@@ -351,7 +366,7 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
         qs.see(item.p, item.with, seen, whole);
 
         const float ks = pow2((int8_t)e);
-        const int ev = (int8_t)(e >> 8), up = ev > unit ? ev : unit;
+        const int ev = (int8_t)(e >> 8), up = unit.follow(ev);
         f32x4 sc[CT][4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -369,8 +384,8 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
         }
         if (following.page >= 0) load_keys(rows_next);
         f16x8 pf[CT][2];
-        weigh<CT, DT>(sc, seen, whole, g, a.c, up, unit, m, l, o, pf);
-        unit = up;
+        weigh<CT, DT>(sc, seen, whole, g, a.c, up, held_unit, m, l, o, pf);
+        held_unit = up;
         const float vs = pow2(ev - up);
         if (!whole) {
             KEEP_BRANCH();
@@ -414,9 +429,9 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
         if (x > 0) __syncthreads();
-        const float u = pow2(unit);
+        const float inv = l[x][0] == 0.f ? 0.f : pow2(held_unit) / l[x][0];  // averages: sums could pass fp32's range
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(so + (wave * 16 + col) * (D + 4) + 16 * d + 4 * g) = o[x][d] * u;
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(so + (wave * 16 + col) * (D + 4) + 16 * d + 4 * g) = o[x][d] * inv;
         if (g == 0) {
             sm[wave * 16 + col] = m[x];
             sl[wave * 16 + col] = l[x][0];
@@ -430,20 +445,21 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
 #pragma unroll
             for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w * 16 + cc]);
             const float ref = top > NEG_INF ? top : 0.f;
-            float total = 0.f;
-            f32x4 v{0.f, 0.f, 0.f, 0.f};
+            float f[W], total = 0.f;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float f = __builtin_amdgcn_exp2f(sm[w * 16 + cc] - ref);
-                total += f * sl[w * 16 + cc];
-                v += *reinterpret_cast<const f32x4*>(so + (w * 16 + cc) * (D + 4) + d) * f;
+                f[w] = __builtin_amdgcn_exp2f(sm[w * 16 + cc] - ref) * sl[w * 16 + cc];
+                total += f[w];
             }
+            const float share = total == 0.f ? 0.f : 1.f / total;
+            f32x4 v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < W; ++w) v += *reinterpret_cast<const f32x4*>(so + (w * 16 + cc) * (D + 4) + d) * (f[w] * share);
             const int64_t r = cs.row_of(y);
             if (a.splits == 1) {
-                const float inv = total == 0.f ? 0.f : 1.f / total;
                 bf16x4 b;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) b[i] = (bf16_t)(v[i] * inv);
+                for (int i = 0; i < 4; ++i) b[i] = (bf16_t)v[i];
                 *reinterpret_cast<bf16x4*>(a.out + r * D + d) = b;
             } else {
                 *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)part * a.rows + r) * D + d) = v;
@@ -517,7 +533,8 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    int unit = ASRK_KV_EXP_MIN, tile_unit = ASRK_KV_EXP_MIN;  // of o, and of the value tiles: the largest exponent so far
+    Unit unit;                 // of the value tiles, alike in all waves
+    int held_unit = unit.now;  // of o
 
     const char* layer = (const char*)c.kv + a.layer * c.num_pages * cs.H * (int64_t)(2 * ASRK_KV_PAGE * D);
     const int* exps = (const int*)c.exps + a.layer * c.num_pages * cs.H;
@@ -549,8 +566,7 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
         const __amdgpu_buffer_rsrc_t rows_next = page_rows(layer, at, D);
         const int e = __builtin_amdgcn_readfirstlane(e_next);
         if (following.page >= 0) e_next = exps[at];
-        const int ev = (int8_t)(e >> 8), up = ev > tile_unit ? ev : tile_unit;
-        tile_unit = up;
+        const int ev = (int8_t)(e >> 8), up = unit.follow(ev);
         const bool odd = __builtin_expect((e >> 16) & 1, 0);
         {
             const float ks = pow2((int8_t)e), vs = pow2(ev - up);
@@ -603,8 +619,8 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
                 }
             }
             f16x8 pf[CT][2];
-            weigh<CT, DT>(sc, seen, whole, g, a.c, up, unit, m, l, o, pf);
-            unit = up;
+            weigh<CT, DT>(sc, seen, whole, g, a.c, up, held_unit, m, l, o, pf);
+            held_unit = up;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -620,14 +636,13 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
         item = following;
         rows = rows_next;
     }
-    const float u = pow2(unit);
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
         const int y = first_col + 16 * x + col;
         if (y >= cs.columns) continue;
         const int64_t r = cs.row_of(y);
+        const float inv = l[x][0] == 0.f ? 0.f : pow2(held_unit) / l[x][0];
         if (a.splits == 1) {
-            const float inv = l[x][0] == 0.f ? 0.f : u / l[x][0];
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 bf16x4 b;
@@ -637,13 +652,13 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
             }
         } else {
 #pragma unroll
-            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)part * a.rows + r) * D + 16 * d + 4 * g) = o[x][d] * u;
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)part * a.rows + r) * D + 16 * d + 4 * g) = o[x][d] * inv;
             if (g == 0) a.part_ml[(int64_t)part * a.rows + r] = make_float2(m[x], l[x][0]);
         }
     }
 }
 
-// Joins the splits: D / 4 lanes per row.
+// Joins the splits (averages, with their maxima and sums of weights): D / 4 lanes per row.
 template <int D>
 __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, int splits,
                                                                 int64_t rows, bf16_t* __restrict__ out) {
@@ -655,19 +670,21 @@ __global__ __launch_bounds__(256) void kv_attention_join_kernel(const float* __r
     for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml[s * rows + r].x);
     const float ref = top > NEG_INF ? top : 0.f;
     float total = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) {
+        const float2 ml = part_ml[s * rows + r];
+        total += __builtin_amdgcn_exp2f(ml.x - ref) * ml.y;
+    }
+    const float share = total == 0.f ? 0.f : 1.f / total;
     f32x4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) {
         const float2 ml = part_ml[s * rows + r];
-        const f32x4 part = *reinterpret_cast<const f32x4*>(part_o + (s * rows + r) * D + d);
-        const float f = __builtin_amdgcn_exp2f(ml.x - ref);
-        total += f * ml.y;
-        v += part * f;
+        v += *reinterpret_cast<const f32x4*>(part_o + (s * rows + r) * D + d) * (__builtin_amdgcn_exp2f(ml.x - ref) * ml.y * share);
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
     bf16x4 y;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = (bf16_t)(v[i] * inv);
+    for (int i = 0; i < 4; ++i) y[i] = (bf16_t)v[i];
     *reinterpret_cast<bf16x4*>(out + r * D + d) = y;
 }
 

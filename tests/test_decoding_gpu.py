@@ -496,6 +496,42 @@ def test_a_write_after_reorder_waits_for_extend():
     same_tokens(c, o, 0, 80)
 
 
+@pytest.mark.parametrize("gap", [16, 30, 60])
+@pytest.mark.parametrize("n,group", [(1, 3), (1, 20), (50, 2)])
+def test_attend_beams_of_very_different_scales(gap, n, group):
+    """Beams whose values are 2**gap apart do not cost each other bits, whichever comes first."""
+    rng = np.random.default_rng(gap)
+    S = 4
+    c, o = both(S, 300, 1, 64)
+    for rows in (130, n):
+        c.extend(rows)
+        o.extend(rows)
+        k, v = (torch.from_numpy(rng.standard_normal((S, rows, 1, 64))).float().cuda() for _ in range(2))
+        v *= torch.tensor([0, gap, -gap / 2, 3], device="cuda").exp2().view(S, 1, 1, 1)
+        c.write(k, v)
+        o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+    q = torch.from_numpy(rng.standard_normal((S, n, group, 64))).cuda().bfloat16()
+    same_attention(c, o, q, beams=S)
+    same_attention(c, o, q, beams=2)
+
+
+@pytest.mark.parametrize("n,max_len", [(1, 300), (1, 4000), (100, 300), (100, 4000)])
+def test_attend_at_the_end_of_the_range(n, max_len):
+    """Values up to 2**127: sums of weighted values would overflow, their averages do not."""
+    rng = np.random.default_rng(n)
+    c, o = both(2, max_len, 1, 64)
+    for rows in (130, n):
+        c.extend(rows)
+        o.extend(rows)
+        k, v = (torch.from_numpy(rng.standard_normal((2, rows, 1, 64))).float().cuda() for _ in range(2))
+        v = v.clamp(-3, 3) * torch.tensor([2.0 ** 125, 2.0 ** 100], device="cuda").view(2, 1, 1, 1)
+        c.write(k, v)
+        o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+    q = torch.from_numpy(rng.standard_normal((2, n, 2, 64))).cuda().bfloat16()
+    same_attention(c, o, q)
+    same_attention(c, o, q, beams=2)
+
+
 def test_attend_takes_any_strides():
     rng = np.random.default_rng(10)
     c, o = filled(rng, 3, 2, 64, [70, 3, 100], [2, 2, 2], layers=2)

@@ -215,11 +215,15 @@ struct Unit {
 // weight of 2^-27 of the largest still has all 11 bits, and below that it is held to 2^-38 of the largest.  The reference
 // follows the maximum only when that has grown by more than 2^SLACK: up to there nothing overflows (2^15) and o and the sum
 // need no rescaling.
+// Where scores pass 2^20 or so, their neighbouring fp32 numbers lie far apart and the reference is off by that much; so it is
+// rounded down, and a weight cut at f16's largest number: scores closer than two of those neighbours then count the same (the cut
+// costs 2 % of the prompts' time; branches for such scores would cost single tokens 10 %).
 constexpr float HEAD = 13.f, SLACK = 2.f;
 template <int CT, int DT>
 __device__ __forceinline__ void weigh(f32x4 (*sc)[4], const int* seen, bool whole, int g, float scale, int up, int unit, float* m, f32x4* l,
                                       f32x4 (*o)[DT], f16x8 (*pf)[2]) {
     const float shrink = pow2(unit - up);
+    constexpr _Float16 MOST = 65504.f;
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
         if (!whole) {
@@ -238,7 +242,8 @@ __device__ __forceinline__ void weigh(f32x4 (*sc)[4], const int* seen, bool whol
         const float now = groups_max(top) * scale;  // scale > 0
         if (__any(now > m[x] + SLACK) || up != unit) {
             KEEP_BRANCH();
-            const float to = now > m[x] + SLACK ? now : m[x];  // by the column alone: its bits do not depend on its neighbours
+            const float low = fmaf(fabsf(now), -0x1p-23f, now);  // +inf: NaN, as the result has to be
+            const float to = now > m[x] + SLACK && !(low <= m[x]) ? low : m[x];  // by the column alone: its bits do not depend on its neighbours
             const float back = to > NEG_INF ? __builtin_amdgcn_exp2f(m[x] - to) : 0.f;
             m[x] = to;
 #pragma unroll
@@ -246,14 +251,14 @@ __device__ __forceinline__ void weigh(f32x4 (*sc)[4], const int* seen, bool whol
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[x][d] *= back * shrink;
         }
-        const float ref = m[x] > NEG_INF ? m[x] - HEAD : 0.f;  // nothing seen yet: every weight is 0
+        const float ref = m[x] == NEG_INF ? 0.f : m[x] - HEAD;  // nothing seen yet: every weight is 0
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
                 const f32x2_t w = {__builtin_amdgcn_exp2f(fmaf(sc[x][t][i], scale, -ref)),
                                    __builtin_amdgcn_exp2f(fmaf(sc[x][t][i + 1], scale, -ref))};
-                const f16x2 h = __builtin_convertvector(w, f16x2);  // to nearest
+                const f16x2 h = __builtin_elementwise_minimum(__builtin_convertvector(w, f16x2), f16x2{MOST, MOST});  // to nearest; NaN stays
                 pf[x][t >> 1][4 * (t & 1) + i] = h[0];
                 pf[x][t >> 1][4 * (t & 1) + i + 1] = h[1];
             }
@@ -473,11 +478,11 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
 // it is vector instructions, and a fifth of those are conversions, so every page is converted once for the four waves: each
 // converts a quarter, into LDS, in the order in which the products' first operands are read (a lane's 16 bytes after
 // another's: no bank conflict).  Two buffers, one barrier per page; the next page's bytes are on their way meanwhile.
-// 16 prompts of up to 1541 tokens, 15 query heads on 5 of 64: 91 us (450 TFLOP/s; every wave converting for itself 105); of 4096
-// tokens 755 TFLOP/s, with heads of 128 860.  Of a wave's vector issue slots 60 % are used: the rest is the prologue of short
+// 16 prompts of up to 1541 tokens, 15 query heads on 5 of 64: 93 us (440 TFLOP/s; every wave converting for itself 105); of 4096
+// tokens 720 TFLOP/s, with heads of 128 830.  Of a wave's vector issue slots 60 % are used: the rest is the prologue of short
 // rows and waves of a workgroup waiting for each other.
 constexpr int PROMPT_W = 4, PROMPT_CT = 2;
-// (D 64: 4 waves per SIMD, a few spilled registers included: 16 prompts of 4096 tokens 684 us; 3 waves 738.)
+// (D 64: 4 waves per SIMD, a few spilled registers included: 16 prompts of 4096 tokens 715 us; 3 waves 738 when it was 684.)
 constexpr int prompt_occupancy(int D) { return D == 64 ? 4 : 2; }
 template <int D>
 __global__ __launch_bounds__(64 * PROMPT_W) __attribute__((amdgpu_waves_per_eu(prompt_occupancy(D), prompt_occupancy(D))))

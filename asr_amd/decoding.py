@@ -168,9 +168,10 @@ class PagedKVCache:
 
     ``max_len`` is rounded up to whole pages; ``num_pages`` is room for all sequences at that length unless it is given.
     The cache and its views belong to one stream at a time.  Its tensors (``kv``, ``exps``, ``table``, ``lens``, ``starts``,
-    ``refs``: the layout is that of ``asrk_kv_cache`` in include/asrk.h) may be read, and overwritten in place; they are
-    never replaced, so a captured step stays valid.  Calls that cannot be carried out on the device (no free page, a
-    sequence longer than ``max_len``) add nothing and set ``status``: ``check()`` raises for it."""
+    ``refs``: the layout is that of ``asrk_kv_cache`` in include/asrk.h) may be read, and overwritten in place by what they
+    held before, all of them together; they are never replaced, so a captured step stays valid.  Calls that cannot be
+    carried out on the device (no free page, a sequence longer than ``max_len``) add nothing and set ``status``:
+    ``check()`` raises for it."""
 
     def __init__(self, num_seqs: int, max_len: int, kv_heads: int, head_dim: int, *, num_layers: int = 1,
                  num_pages: Optional[int] = None, device: Union[str, torch.device] = "cuda"):

@@ -532,6 +532,41 @@ def test_attend_at_the_end_of_the_range(n, max_len):
     same_attention(c, o, q, beams=2)
 
 
+@pytest.mark.parametrize("power", [16, 30, 100])
+@pytest.mark.parametrize("n,max_len", [(1, 300), (1, 4000), (100, 300), (100, 4000)])
+def test_attend_with_enormous_scores(n, max_len, power):
+    """Scores whose neighbouring fp32 numbers lie far apart: the largest wins, and equal ones share.  Keys of +-2**power and
+    small integers in q, so that every score is exact and ties are ties."""
+    rng = np.random.default_rng(n + power)
+    c, o = both(3, max_len, 1, 64)
+    for rows in (130, n):
+        c.extend(rows)
+        o.extend(rows)
+        k, v = (torch.from_numpy(x).float().cuda() for x in (rng.choice([-1.0, 1.0], (3, rows, 1, 64)) * 2.0 ** power, rng.standard_normal((3, rows, 1, 64))))
+        c.write(k, v)
+        o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+    q = torch.from_numpy(rng.integers(-3, 4, (3, n, 2, 64))).cuda().bfloat16()
+    q[1, :, 1] *= 2.0 ** -power  # beside ordinary ones
+    q[2, :, 0] = 1
+    same_attention(c, o, q)
+    same_attention(c, o, q, beams=3)
+
+
+@pytest.mark.parametrize("n", [1, 100])
+def test_attend_keeps_the_queries_nan(n):
+    """A query with a NaN or an infinity gives NaN, and changes no other row."""
+    rng = np.random.default_rng(n)
+    c, o = filled(rng, 2, 1, 64, [130, 200], [n, n])
+    q = torch.from_numpy(rng.standard_normal((2, n, 3, 64))).cuda().bfloat16()
+    clean = c.attend(q)
+    q[0, n // 2, 1, 5], q[1, n - 1, 0, 9], q[1, 0, 2, 60] = float("nan"), float("inf"), float("-inf")
+    with np.errstate(invalid="ignore"):
+        same_attention(c, o, q)
+    got = c.attend(q)
+    hit = torch.isnan(q).any(-1) | torch.isinf(q).any(-1)
+    assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], clean[~hit])
+
+
 def test_attend_takes_any_strides():
     rng = np.random.default_rng(10)
     c, o = filled(rng, 3, 2, 64, [70, 3, 100], [2, 2, 2], layers=2)

@@ -16,24 +16,27 @@ namespace {
 
 constexpr int MANAGE_T = 1024;  // threads of the one-workgroup kernels
 
-__device__ __forceinline__ int block_scan_exclusive(int v, int* lds, int& total) {  // MANAGE_T threads
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
+// Inclusive sums over a wave, or over its first 16 lanes (ROW): shifts within rows of 16, then rows broadcast to later ones.
+template <bool ROW>
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    if (!ROW) {
+        x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
     }
+    return x;
+}
+__device__ __forceinline__ int block_scan_exclusive(int v, int* lds, int& total) {  // MANAGE_T threads, 16 waves
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = wave_scan<false>(v);
     if (lane == 63) lds[wave] = x;
     __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < MANAGE_T / 64; ++w) {
-        const int t = lds[w];
-        before += w < wave ? t : 0;
-        total += t;
-    }
+    const int w = lds[lane & 15], upto = wave_scan<true>(w);
+    total = __builtin_amdgcn_readlane(upto, 15);
+    const int before = __builtin_amdgcn_readlane(upto, wave) - __builtin_amdgcn_readlane(w, wave);
     __syncthreads();
     return before + x - v;
 }
@@ -60,33 +63,30 @@ struct Scratch {
     }
 };
 
-// Lists up to `want` pages, in ascending order from `from` (below `to`), whose holders are none (FREE) or some; returns how many there are.
-template <bool FREE>
-__device__ int list_pages(const int* refs, int from, int to, int want, int* out, int* lds) {
-    constexpr int PER = 16;
+// The holders of four pages from `at` on.
+constexpr int LIST_PER = 4;
+struct Refs {
+    int r[LIST_PER];
+    __device__ __forceinline__ void load(const int* refs, int at, int to) {
+#pragma unroll
+        for (int i = 0; i < LIST_PER; ++i) r[i] = at + i < to ? refs[at + i] : -1;
+    }
+};
+
+// Lists up to `want` pages, in ascending order from `from` (below `to`), whose holders are none (FREE) or some: put(place, page);
+// returns how many there are.  `held`: of this thread's pages from `from` on.
+template <bool FREE, class Put>
+__device__ __forceinline__ int list_pages(const int* refs, Refs held, int from, int to, int want, int* lds, Put&& put) {
     int found = 0;
-    for (int base = from; base < to && found < want; base += MANAGE_T * PER) {
-        const int at = base + threadIdx.x * PER;
+    for (int base = from; base < to && found < want; base += MANAGE_T * LIST_PER) {
+        const int at = base + threadIdx.x * LIST_PER;
+        if (base > from) held.load(refs, at, to);
         uint32_t mine = 0;
-        if (at + PER <= to && !(((uintptr_t)(refs + at)) & 15)) {
-            u32x4 r[PER / 4];
 #pragma unroll
-            for (int i = 0; i < PER / 4; ++i) r[i] = reinterpret_cast<const u32x4*>(refs + at)[i];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) mine |= (FREE == (r[i / 4][i % 4] == 0) ? 1u : 0u) << i;
-        } else {
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (at + i < to) mine |= (FREE == (refs[at + i] == 0) ? 1u : 0u) << i;
-        }
+        for (int i = 0; i < LIST_PER; ++i) mine |= (FREE ? held.r[i] == 0 : held.r[i] > 0) ? 1u << i : 0;
         int total;
         int r = found + block_scan_exclusive(__popc(mine), lds, total);
-        while (mine) {
-            const int i = __builtin_ctz(mine);
-            mine &= mine - 1;
-            if (r < want) out[r] = at + i;
-            ++r;
-        }
+        for (; mine && r < want; mine &= mine - 1, ++r) put(r, at + __builtin_ctz(mine));
         found += total;
     }
     return found < want ? found : want;
@@ -95,89 +95,130 @@ __device__ int list_pages(const int* refs, int from, int to, int want, int* out,
 // Room for n[s] more tokens of every sequence: the lowest free pages, in the order of the sequences, and a page of its
 // own for a sequence that writes into one it shares -- the first of its holders keeps it if they all write.  All or
 // nothing: without enough pages (or with a count that does not fit) nothing is added and `status` says so.  One
-// workgroup: the work is a few integers per sequence and the order has to be total; bound by its chain of dependent accesses,
-// 7 us for 5 sequences and 10 for 160, once per step for all layers.
+// workgroup: the work is a few integers per sequence and the order has to be total.  Bound by its chain of dependent accesses
+// and by instructions that are fetched for the first time (the cache for them is cold: 1 to 1.5 us per KB of code that runs).
+// So a sequence per thread (SMALL) is held in registers and LDS from one step to the next, the first pages' holders are on
+// their way from the start, and nothing is unrolled that need not be: 3.7 us for a step of 5 sequences, 4.8 of 160 that share
+// their pages (through memory, and with twice the code, 7 and 10), once per step for all layers.
+template <bool SMALL>  // at most MANAGE_T sequences
 __global__ __launch_bounds__(MANAGE_T) void kv_extend_kernel(asrk_kv_cache c, const int* __restrict__ n_each, int n_all) {
     __shared__ int lds[MANAGE_T / 64];
+    __shared__ int shared_page[SMALL ? 2 * MANAGE_T : 1], writers[SMALL ? 2 * MANAGE_T : 1], lowest[SMALL ? 2 * MANAGE_T : 1];  // hashed, -1: none
+    __shared__ int fresh[MANAGE_T];  // the pages handed out, if they are few
     __shared__ int flags, n_moves;
     Scratch sc(c.scratch, c.num_pages, (int64_t)c.num_seqs * c.seq_stride);
     const int S = c.num_seqs, M = c.max_pages;
-    if (threadIdx.x == 0) { flags = 0; n_moves = 0; }
-    __syncthreads();
-    for (int s = threadIdx.x; s < S; s += MANAGE_T) {  // who writes into which open page
+    struct Seq {
+        int len, n, page, refs;  // page: the open one, if it is written into
+    };
+    auto load = [&](int s) -> Seq {
         const int64_t slot = (int64_t)s * c.seq_stride;
-        const int len = c.lens[slot], n = n_each ? n_each[s] : n_all;
-        if (n < 0) atomicOr(&flags, ASRK_KV_BAD_COUNT);
-        else if (n > (int64_t)M * ASRK_KV_PAGE - len) atomicOr(&flags, ASRK_KV_TOO_LONG);
-        else if (n > 0) {
-            const int page = open_page(c, slot, len);
-            if (page >= 0) {
-                atomicAdd(&sc.writers[page], 1);
-                atomicMax(&sc.lowest[page], S - s);
-            }
+        Seq q{c.lens[slot], n_each ? n_each[s] : n_all, -1, 0};
+        if (q.n > 0 && q.n <= M * ASRK_KV_PAGE - q.len) q.page = open_page(c, slot, q.len);
+        if (q.page >= 0) q.refs = c.refs[q.page];
+        return q;
+    };
+    Refs first;
+    first.load(c.refs, threadIdx.x * LIST_PER, c.num_pages);
+    if (threadIdx.x == 0) { flags = 0; n_moves = 0; }
+    Seq mine{0, 0, -1, 0};
+    if (SMALL && (int)threadIdx.x < S) mine = load(threadIdx.x);
+    auto seq = [&](int s) -> Seq { return SMALL ? mine : load(s); };
+    if (SMALL)
+#pragma unroll
+        for (int i = 0; i < 2 * MANAGE_T; i += MANAGE_T) {
+            shared_page[i + threadIdx.x] = -1;
+            writers[i + threadIdx.x] = lowest[i + threadIdx.x] = 0;
+        }
+    __syncthreads();
+    int place = 0;
+    if (SMALL && mine.refs > 1) {  // at most half of the places are taken
+        place = (uint32_t)mine.page * 0x9e3779b1u >> 21;
+        for (;; place = (place + 1) % (2 * MANAGE_T)) {
+            const int there = atomicCAS(&shared_page[place], -1, mine.page);
+            if (there == -1 || there == mine.page) break;
+        }
+        atomicAdd(&writers[place], 1);
+        atomicMax(&lowest[place], S - (int)threadIdx.x);
+    }
+    for (int s = threadIdx.x; s < S; s += MANAGE_T) {  // who writes into which open page
+        const Seq q = seq(s);
+        if (q.n < 0) atomicOr(&flags, ASRK_KV_BAD_COUNT);
+        else if (q.n > M * ASRK_KV_PAGE - q.len) atomicOr(&flags, ASRK_KV_TOO_LONG);
+        else if (!SMALL && q.page >= 0) {
+            atomicAdd(&sc.writers[q.page], 1);
+            atomicMax(&sc.lowest[q.page], S - s);
         }
     }
     __syncthreads();  // one workgroup: its atomics are done (at L2) and are read there, past L1
     const bool fits = flags == 0;
-    __syncthreads();
-    int need_all = 0;
+    int need_all = 0, my_begin = 0, my_copy = 0;
     for (int base = 0; base < S && fits; base += MANAGE_T) {
         const int s = base + threadIdx.x;
         int need = 0, copy = 0;
         if (s < S) {
-            const int64_t slot = (int64_t)s * c.seq_stride;
-            const int len = c.lens[slot], n = n_each ? n_each[s] : n_all;
-            need = (len + n + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE - (len + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
-            const int page = n > 0 ? open_page(c, slot, len) : -1;
-            if (page >= 0) {
-                const int refs = c.refs[page];
-                copy = refs > 1 && !(load_agent(&sc.writers[page]) == refs && load_agent(&sc.lowest[page]) == S - s);
+            const Seq q = seq(s);
+            need = (q.len + q.n + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE - (q.len + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
+            if (q.page >= 0 && q.refs > 1) {
+                const int all = SMALL ? writers[place] : load_agent(&sc.writers[q.page]);
+                const int lead = SMALL ? lowest[place] : load_agent(&sc.lowest[q.page]);
+                copy = !(all == q.refs && lead == S - s);
             }
             need += copy;
         }
         int total;
         const int begin = need_all + block_scan_exclusive(need, lds, total);
-        if (s < S) {
+        if (SMALL) {
+            my_begin = begin;
+            my_copy = copy;
+        } else if (s < S) {
             sc.tmp[2 * s] = begin;
             sc.tmp[2 * s + 1] = copy;
         }
         need_all += total;
     }
     int got = 0;
+    const bool few = need_all <= MANAGE_T;
     if (fits && need_all > 0) {
-        got = need_all <= c.num_pages ? list_pages<true>(c.refs, 0, c.num_pages, need_all, sc.list, lds) : 0;
+        got = need_all <= c.num_pages ? list_pages<true>(c.refs, first, 0, c.num_pages, need_all, lds,
+                                                         [&](int r, int page) {
+                                                             if (few) fresh[r] = page;
+                                                             else sc.list[r] = page;
+                                                         })
+                                      : 0;
         if (got < need_all && threadIdx.x == 0) flags = ASRK_KV_OUT_OF_PAGES;
         __syncthreads();
     }
     const bool go = fits && got == need_all;
+    auto handed = [&](int i) { return few ? fresh[i] : load_agent(&sc.list[i]); };
     for (int s = threadIdx.x; s < S; s += MANAGE_T) {
         const int64_t slot = (int64_t)s * c.seq_stride;
-        const int len = c.lens[slot], n = n_each ? n_each[s] : n_all;
+        const Seq q = seq(s);
+        const int begin = SMALL ? my_begin : sc.tmp[2 * s], copy = SMALL ? my_copy : sc.tmp[2 * s + 1];
         int* row = c.table + slot * M;
-        const int page = n > 0 && n <= (int64_t)M * ASRK_KV_PAGE - len ? open_page(c, slot, len) : -1;
-        if (page >= 0) {
-            sc.writers[page] = 0;
-            sc.lowest[page] = 0;
-            if (go && sc.tmp[2 * s + 1]) {
-                const int own = load_agent(&sc.list[sc.tmp[2 * s]]);
-                row[len / ASRK_KV_PAGE] = own;
-                c.refs[own] = 1;
-                atomicSub(&c.refs[page], 1);
-                const int m = atomicAdd(&n_moves, 1);
-                sc.moves[2 * m] = page;
-                sc.moves[2 * m + 1] = own;
-            }
+        if (!SMALL && q.page >= 0) {
+            sc.writers[q.page] = 0;
+            sc.lowest[q.page] = 0;
         }
         if (go) {
-            int at = sc.tmp[2 * s] + sc.tmp[2 * s + 1];
-            for (int j = (len + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE; j < (len + n + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE; ++j, ++at) {
-                const int own = load_agent(&sc.list[at]);
+            if (copy) {
+                const int own = handed(begin);
+                row[q.len / ASRK_KV_PAGE] = own;
+                c.refs[own] = 1;
+                atomicSub(&c.refs[q.page], 1);
+                const int m = atomicAdd(&n_moves, 1);
+                sc.moves[2 * m] = q.page;
+                sc.moves[2 * m + 1] = own;
+            }
+            int at = begin + copy;
+            for (int j = (q.len + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE; j < (q.len + q.n + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE; ++j, ++at) {
+                const int own = handed(at);
                 row[j] = own;
                 c.refs[own] = 1;
             }
-            c.lens[slot] = len + n;
+            c.lens[slot] = q.len + q.n;
         }
-        c.starts[slot] = len;  // also if nothing was added: then no row is new
+        c.starts[slot] = q.len;  // also if nothing was added: then no row is new
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -204,48 +245,31 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(asrk_kv_cache c) {
 }
 
 // Beam k of group b goes on from beam parents[b][k] of the same group (-1: from nothing, its pages are given back).
-// A thread owns one column of the group's table rows and reads all of it before it writes: in place, in one launch (4 us for
-// 5 sequences, 6 for 160).
+// A workgroup owns some columns of the group's table rows, a thread one entry: all is read before anything is written, in place,
+// in one launch (1.7 us for 5 sequences, 4.8 for 160; a thread per column with its beams unrolled, 16 times the code, 4.0 and 6.4).
 constexpr int REORDER_MAX = 32;
-__global__ __launch_bounds__(64) void kv_reorder_kernel(asrk_kv_cache c, const int64_t* __restrict__ parents, int K) {
-    const int b = blockIdx.y;
-    const int M = c.max_pages;
-    const int j = blockIdx.x * 64 + threadIdx.x;
-    const int64_t* par = parents + (int64_t)b * K;
-    const int64_t first = (int64_t)b * K * c.seq_stride;
-    if (j < M) {
-        int now[REORDER_MAX], then[REORDER_MAX];
-#pragma unroll
-        for (int k = 0; k < REORDER_MAX; ++k)
-            if (k < K) {
-                const int64_t p = par[k];
-                now[k] = c.table[(first + (int64_t)k * c.seq_stride) * M + j];
-                then[k] = p == -1 ? -1 : (p < 0 || p >= K ? now[k] : c.table[(first + p * c.seq_stride) * M + j]);
-            }
-#pragma unroll
-        for (int k = 0; k < REORDER_MAX; ++k)
-            if (k < K && now[k] != then[k]) {
-                c.table[(first + (int64_t)k * c.seq_stride) * M + j] = then[k];
-                if (then[k] >= 0) atomicAdd(&c.refs[then[k]], 1);
-                if (now[k] >= 0) atomicSub(&c.refs[now[k]], 1);
-            }
+__global__ __launch_bounds__(1024) void kv_reorder_kernel(asrk_kv_cache c, const int64_t* __restrict__ parents, int K, int log_columns) {
+    const int b = blockIdx.y, k = threadIdx.x >> log_columns, j = (blockIdx.x << log_columns) + (threadIdx.x & ((1 << log_columns) - 1));
+    const int64_t par = parents[(int64_t)b * K + k], first = (int64_t)b * K * c.seq_stride;
+    const bool known = par >= 0 && par < K, gone = par == -1;
+    const int64_t slot = first + (int64_t)k * c.seq_stride, from = known ? first + par * c.seq_stride : slot;
+    int* entry = c.table + slot * c.max_pages + j;
+    int now = -1, then = -1, len = 0;
+    if (j < c.max_pages) {
+        now = *entry;
+        then = gone ? -1 : c.table[from * c.max_pages + j];
     }
-    if (blockIdx.x == 0) {  // one wave: all lengths are read before any is written
-        const int k = threadIdx.x;
-        int len = 0;
-        if (k < K) {
-            int64_t p = par[k];
-            if (p < -1 || p >= K) {
-                atomicOr(&c.status[0], ASRK_KV_BAD_PARENT);
-                p = k;
-            }
-            if (p >= 0) len = c.lens[first + p * c.seq_stride];
-        }
-        __syncthreads();
-        if (k < K) {
-            c.lens[first + (int64_t)k * c.seq_stride] = len;
-            c.starts[first + (int64_t)k * c.seq_stride] = len;  // no token is new: a write before the next extend could meet a shared page
-        }
+    if (j == 0 && !gone) len = c.lens[from];
+    __syncthreads();
+    if (now != then) {
+        *entry = then;
+        if (then >= 0) atomicAdd(&c.refs[then], 1);
+        if (now >= 0) atomicSub(&c.refs[now], 1);
+    }
+    if (j == 0) {
+        if (!known && !gone) atomicOr(&c.status[0], ASRK_KV_BAD_PARENT);
+        c.lens[slot] = len;
+        c.starts[slot] = len;  // no token is new: a write before the next extend could meet a shared page
     }
 }
 
@@ -263,8 +287,11 @@ __global__ __launch_bounds__(MANAGE_T) void kv_compact_plan_kernel(asrk_kv_cache
     block_scan_exclusive(mine, lds, used);
     int* holes = sc.writers;  // both are zero between calls; they are cleared again below
     int* high = sc.lowest;
-    const int n = list_pages<true>(c.refs, 0, used, used, holes, lds);
-    list_pages<false>(c.refs, used, P, n, high, lds);
+    Refs first;
+    first.load(c.refs, threadIdx.x * LIST_PER, used);
+    const int n = list_pages<true>(c.refs, first, 0, used, used, lds, [&](int r, int page) { holes[r] = page; });
+    first.load(c.refs, used + threadIdx.x * LIST_PER, P);
+    list_pages<false>(c.refs, first, used, P, n, lds, [&](int r, int page) { high[r] = page; });
     __syncthreads();
     for (int r = threadIdx.x; r < n; r += MANAGE_T) {
         const int src = load_agent(&high[r]), dst = load_agent(&holes[r]);
@@ -590,7 +617,8 @@ extern "C" int asrk_kv_extend(const asrk_kv_cache* c, const int32_t* n_each, int
     if (int rc = asrk_kv_check(c)) return rc;
     if (!n_each && n_all < 0) return ASRK_ERR_SHAPE;
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(kv_extend_kernel, dim3(1), dim3(MANAGE_T), 0, st, *c, n_each, n_all);
+    if (c->num_seqs <= MANAGE_T) hipLaunchKernelGGL(kv_extend_kernel<true>, dim3(1), dim3(MANAGE_T), 0, st, *c, n_each, n_all);
+    else hipLaunchKernelGGL(kv_extend_kernel<false>, dim3(1), dim3(MANAGE_T), 0, st, *c, n_each, n_all);
     launch_copies(c, c->num_seqs, st);
     return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
 }
@@ -599,7 +627,9 @@ extern "C" int asrk_kv_reorder(const asrk_kv_cache* c, const int64_t* parents, i
     if (int rc = asrk_kv_check(c)) return rc;
     if (!parents) return ASRK_ERR_NULL;
     if (K <= 0 || K > REORDER_MAX || c->num_seqs % K) return ASRK_ERR_SHAPE;
-    hipLaunchKernelGGL(kv_reorder_kernel, dim3((c->max_pages + 63) / 64, c->num_seqs / K), dim3(64), 0, (hipStream_t)stream, *c, parents, K);
+    const int log_columns = K <= 16 ? 6 : 5, columns = 1 << log_columns;
+    hipLaunchKernelGGL(kv_reorder_kernel, dim3((c->max_pages + columns - 1) / columns, c->num_seqs / K), dim3(columns * K), 0, (hipStream_t)stream, *c,
+                       parents, K, log_columns);
     return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
 }
 

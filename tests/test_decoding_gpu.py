@@ -280,6 +280,29 @@ def test_pages_of_thousands_of_sequences():
     assert o.status in (0, 2)
 
 
+@pytest.mark.parametrize("B,K", [(32, 32), (41, 25), (512, 2), (128, 8), (1000, 1), (3, 17)])
+@pytest.mark.parametrize("pages", [700, 2500, 9000])
+def test_pages_shared_by_many(B, K, pages):
+    """About as many sequences as the workgroup has threads, pages with up to 32 holders of which all, some or one write, and
+    steps that hand out more pages than the workgroup has threads."""
+    rng = np.random.default_rng(1000 * pages + 10 * B + K)
+    c, o = both(B * K, 320, 1, 64, pages=pages)
+    lead = c.leaders(K)
+    n = rng.integers(0, 130, B)
+    lead.extend(torch.from_numpy(n).cuda())
+    o.extend(n, K)
+    same_pages(c, o)
+    for step in range(4):
+        par = np.zeros((B, K), np.int64) if step == 0 else rng.integers(-1, K, (B, K))
+        c.reorder(torch.from_numpy(par).cuda())
+        o.reorder(par)
+        same_pages(c, o)
+        for n in (rng.integers(0, 2, B * K), np.ones(B * K, np.int64), rng.integers(0, 100, B * K)):
+            c.extend(torch.from_numpy(n).cuda())
+            o.extend(n)
+            same_pages(c, o)
+
+
 def test_what_does_not_fit_adds_nothing_and_is_reported():
     from asr_amd import _lib
 

@@ -36,7 +36,8 @@ struct AttnArgs {
     float* part_o;   // [splits][S n Hq][D]
     float2* part_ml; // [splits][S n Hq]
     int64_t seq_ld, row_ld, head_ld, layer, rows;  // rows: S n Hq
-    int n, group, beams, splits, chunks, sets;  // new tokens, query heads per key/value head, ..., groups of beams
+    double per_seq_inv, group_inv;  // 1 / (n group), 1 / group: a division by a runtime integer is 30 instructions
+    int n, group, beams, splits;    // new tokens, query heads per key/value head
     float c;
 };
 
@@ -70,26 +71,33 @@ __device__ __forceinline__ float groups_max(float v) {  // rows of 16 lanes, the
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ int wave_imax(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const int y = __shfl_xor(v, o, 64);
-        v = v > y ? v : y;
-    }
-    return v;
+__device__ __forceinline__ int larger(int a, int b) { return a > b ? a : b; }
+__device__ __forceinline__ int wave_imax(int v) {  // v >= 0; shifts within rows of 16, then rows broadcast to later ones
+    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(v, 63);
 }
+__device__ __forceinline__ int over(int x, double inverse) { return (int)(((double)x + 0.5) * inverse); }  // exact
+
+// Grid: x: (head, split), y: set of sequences, z: chunk of columns; whole waves in this order.
+__device__ __forceinline__ int head_of(const AttnArgs& a) { return a.splits == 1 ? blockIdx.x : blockIdx.x / (unsigned)a.splits; }
+__device__ __forceinline__ int part_of(const AttnArgs& a) { return a.splits == 1 ? 0 : blockIdx.x % (unsigned)a.splits; }
 
 // Column y of a set of sequences: beam, new token, query head.
 struct Columns {
     const AttnArgs& a;
     int set, h, H, per_seq, columns;
     __device__ __forceinline__ Columns(const asrk_kv_cache& c, const AttnArgs& args, int set_)
-        : a(args), set(set_), h(blockIdx.x / args.splits % c.kv_heads), H(c.kv_heads), per_seq(args.n * args.group), columns(args.beams * per_seq) {}
+        : a(args), set(set_), h(head_of(args)), H(c.kv_heads), per_seq(args.n * args.group), columns(args.beams * per_seq) {}
     __device__ __forceinline__ void split(int y, int& b, int& i, int& j) const {
-        b = a.beams == 1 ? 0 : (int)((unsigned)y / (unsigned)per_seq);
-        const unsigned in = (unsigned)(y - b * per_seq);
-        i = a.n == 1 ? 0 : (int)(in / (unsigned)a.group);
-        j = (int)in - i * a.group;
+        b = over(y, a.per_seq_inv);
+        const int in = y - b * per_seq;
+        i = over(in, a.group_inv);
+        j = in - i * a.group;
     }
     __device__ __forceinline__ int64_t row_of(int y) const {  // of out, in units of D
         int b, i, j;
@@ -301,6 +309,16 @@ __device__ __forceinline__ void mark_nans(Load&& raw_value, const int* seen, int
     }
 }
 
+// f over groups of W lanes, in all of them.
+template <int W, class F>
+__device__ __forceinline__ float among(float v, F&& f) {
+    auto lanes = [&](auto control) { return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), control.value, 0xf, 0xf, true)); };
+    v = f(v, lanes(std::integral_constant<int, 0xB1>()));                   // 1 0 3 2
+    v = f(v, lanes(std::integral_constant<int, 0x4E>()));                   // 2 3 0 1
+    if (W == 8) v = f(v, lanes(std::integral_constant<int, 0x141>()));      // 7 6 5 4 3 2 1 0
+    return v;
+}
+
 // Waves per SIMD that the registers are cut for: as many as hold a page, q, o and the scores without spilling in the loop.
 // (D 64, 1 tile: 4; with 3, 64 x 5 beams take 24.5 us instead of 19.7.  D 128, 1 tile: 2; with 3 it spills and 1.2 GB of
 // cache take 228 us instead of 204.)
@@ -316,14 +334,14 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     constexpr int DT = D / 16;   // tiles of 16 d
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int part = blockIdx.x % a.splits, block = blockIdx.x / a.splits / c.kv_heads, set = block % a.sets;
+    const int part = part_of(a), set = blockIdx.y;
     const Columns cs(c, a, set);
-    const int first_col = block / a.sets * 16 * CT;
+    const int first_col = blockIdx.z * 16 * CT;
     // The pages of a wave: by its number alone, so that their numbers are on the way before the lengths are known.
     Pages work(c, a.beams, set, part * W + wave, a.splits * W);
     Queries<D, CT> qs;
     qs.load(c, cs, first_col, col, g);
-    const int pages = (__builtin_amdgcn_readfirstlane(wave_imax(qs.most)) + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
+    const int pages = ((wave_imax(qs.most)) + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
 
     f32x4 o[CT][DT], l[CT];
     float m[CT];
@@ -427,39 +445,37 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
         rows = rows_next;
     }
 
-    // ---- join the waves, one column tile at a time: thread: column cc, four d's from d on
-    extern __shared__ float shared[];  // so [W][16][D + 4], sm [W][16], sl [W][16]
+    // ---- join the waves, one column tile at a time
+    extern __shared__ float shared[];  // so [W][16][D + 4], sm [16][W], sl [16][W]
     float *so = shared, *sm = so + W * 16 * (D + 4), *sl = sm + W * 16;
     constexpr int PER = D / 4;  // threads per column
 #pragma unroll
     for (int x = 0; x < CT; ++x) {
         if (x > 0) __syncthreads();
-        const float inv = l[x][0] == 0.f ? 0.f : pow2(held_unit) / l[x][0];  // averages: sums could pass fp32's range
+        const float inv = l[x][0] == 0.f ? 0.f : pow2(held_unit) * __builtin_amdgcn_rcpf(l[x][0]);  // averages: sums could pass fp32's range
 #pragma unroll
         for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(so + (wave * 16 + col) * (D + 4) + 16 * d + 4 * g) = o[x][d] * inv;
         if (g == 0) {
-            sm[wave * 16 + col] = m[x];
-            sl[wave * 16 + col] = l[x][0];
+            sm[col * W + wave] = m[x];
+            sl[col * W + wave] = l[x][0];
         }
         __syncthreads();
-        for (int cc = threadIdx.x / PER; cc < 16; cc += 64 * W / PER) {
+        if (threadIdx.x < 16 * W) {  // thread (column, wave): the wave's share of the column
+            const int cc = threadIdx.x / W, y = first_col + 16 * x + cc;
+            const float mine = sm[threadIdx.x], top = among<W>(mine, [](float p, float q) { return fmaxf(p, q); });
+            const float f = __builtin_amdgcn_exp2f(mine - (top > NEG_INF ? top : 0.f)) * sl[threadIdx.x];
+            const float total = among<W>(f, [](float p, float q) { return p + q; });
+            sl[threadIdx.x] = total == 0.f ? 0.f : f * __builtin_amdgcn_rcpf(total);
+            if (a.splits > 1 && threadIdx.x % W == 0 && y < cs.columns) a.part_ml[(int64_t)part * a.rows + cs.row_of(y)] = make_float2(top, total);
+        }
+        __syncthreads();
+        for (int cc = threadIdx.x / PER; cc < 16; cc += 64 * W / PER) {  // thread: column cc, four d's
             const int d = 4 * (threadIdx.x % PER);
             const int y = first_col + 16 * x + cc;
             if (y >= cs.columns) break;
-            float top = NEG_INF;
-#pragma unroll
-            for (int w = 0; w < W; ++w) top = fmaxf(top, sm[w * 16 + cc]);
-            const float ref = top > NEG_INF ? top : 0.f;
-            float f[W], total = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                f[w] = __builtin_amdgcn_exp2f(sm[w * 16 + cc] - ref) * sl[w * 16 + cc];
-                total += f[w];
-            }
-            const float share = total == 0.f ? 0.f : 1.f / total;
             f32x4 v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < W; ++w) v += *reinterpret_cast<const f32x4*>(so + (w * 16 + cc) * (D + 4) + d) * (f[w] * share);
+            for (int w = 0; w < W; ++w) v += *reinterpret_cast<const f32x4*>(so + (w * 16 + cc) * (D + 4) + d) * sl[cc * W + w];
             const int64_t r = cs.row_of(y);
             if (a.splits == 1) {
                 bf16x4 b;
@@ -468,7 +484,6 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
                 *reinterpret_cast<bf16x4*>(a.out + r * D + d) = b;
             } else {
                 *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)part * a.rows + r) * D + d) = v;
-                if (d == 0) a.part_ml[(int64_t)part * a.rows + r] = make_float2(top, total);
             }
         }
     }
@@ -494,7 +509,7 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     // The last rows of every prompt first: they see the most, and what is left for the end is short.
-    const int part = blockIdx.x % a.splits, block = blockIdx.x / a.splits / c.kv_heads, set = block % a.sets, chunk = a.chunks - 1 - block / a.sets;
+    const int part = part_of(a), set = blockIdx.y, chunk = gridDim.z - 1 - blockIdx.z;
     const Columns cs(c, a, set);
     const int first_col = (chunk * W + wave) * 16 * CT;
     Pages work(c, a.beams, set, part, a.splits);
@@ -506,10 +521,10 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
     if (a.beams == 1) {
         const int start = c.starts[seq * c.seq_stride], fresh = __builtin_amdgcn_readfirstlane(held_by) - start;
         const int x0 = chunk * W * 16 * CT, x1 = x0 + W * 16 * CT < cs.columns ? x0 + W * 16 * CT : cs.columns;
-        const int i0 = (int)((unsigned)x0 / (unsigned)a.group), i1 = (int)((unsigned)(x1 - 1) / (unsigned)a.group) + 1;
+        const int i0 = over(x0, a.group_inv), i1 = over(x1 - 1, a.group_inv) + 1;
         most = i0 >= fresh ? 0 : start + (i1 < fresh ? i1 : fresh);
     } else {
-        most = __builtin_amdgcn_readfirstlane(wave_imax(held_by));
+        most = (wave_imax(held_by));
     }
     int pages = (most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
     pages = pages < c.max_pages ? pages : c.max_pages;
@@ -576,7 +591,7 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
         {
             const float ks = pow2((int8_t)e), vs = pow2(ev - up);
             const int held = (a.beams == 1 ? __builtin_amdgcn_readfirstlane(held_by)
-                                           : __builtin_amdgcn_readfirstlane(wave_imax((item.with >> lane) & 1 ? held_by : 0))) - item.p * ASRK_KV_PAGE;
+                                           : (wave_imax((item.with >> lane) & 1 ? held_by : 0))) - item.p * ASRK_KV_PAGE;
             if (held < ASRK_KV_PAGE) {  // the sequence ends within the page
                 KEEP_BRANCH();
                 const u32x4 mask = keep_before(held, g);
@@ -646,7 +661,7 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
         const int y = first_col + 16 * x + col;
         if (y >= cs.columns) continue;
         const int64_t r = cs.row_of(y);
-        const float inv = l[x][0] == 0.f ? 0.f : pow2(held_unit) / l[x][0];
+        const float inv = l[x][0] == 0.f ? 0.f : pow2(held_unit) * __builtin_amdgcn_rcpf(l[x][0]);
         if (a.splits == 1) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
@@ -722,30 +737,30 @@ Plan plan_of(const asrk_kv_cache* c, int n, int q_heads, int beams) {
 }
 
 template <class K>
-int launch(K kernel, const asrk_kv_cache* c, const AttnArgs& a, int threads, int lds, int blocks, std::atomic<uint64_t>& done, hipStream_t st) {
+int launch(K kernel, const asrk_kv_cache* c, const AttnArgs& a, int threads, int lds, int chunks, std::atomic<uint64_t>& done, hipStream_t st) {
     if (lds > 60000)  // beside what the kernel declares itself, 64 KiB need asking for
         if (int rc = asrk_max_lds_once((const void*)kernel, lds, done)) return rc;
-    hipLaunchKernelGGL(kernel, dim3(blocks * c->kv_heads * a.splits), dim3(threads), lds, st, *c, a);
+    hipLaunchKernelGGL(kernel, dim3(c->kv_heads * a.splits, c->num_seqs / a.beams, chunks), dim3(threads), lds, st, *c, a);
     return ASRK_OK;
 }
 template <int D, int CT, int W>
-int launch_shared(const asrk_kv_cache* c, const AttnArgs& a, int blocks, hipStream_t st) {
+int launch_shared(const asrk_kv_cache* c, const AttnArgs& a, int chunks, hipStream_t st) {
     static std::atomic<uint64_t> done{0};
-    return launch(kv_attention_kernel<D, CT, W>, c, a, 64 * W, (W * 16 * (D + 4) + 2 * W * 16) * (int)sizeof(float), blocks, done, st);
+    return launch(kv_attention_kernel<D, CT, W>, c, a, 64 * W, (W * 16 * (D + 4) + 2 * W * 16) * (int)sizeof(float), chunks, done, st);
 }
 template <int D>
-int launch_for(const asrk_kv_cache* c, const AttnArgs& a, const Plan& p, int sets, hipStream_t st) {
+int launch_for(const asrk_kv_cache* c, const AttnArgs& a, const Plan& p, hipStream_t st) {
     if (p.prompt) {
         static std::atomic<uint64_t> done{0};
-        return launch(kv_prompt_kernel<D>, c, a, 64 * PROMPT_W, 4 * ASRK_KV_PAGE * D * 2, sets * p.chunks, done, st);
+        return launch(kv_prompt_kernel<D>, c, a, 64 * PROMPT_W, 4 * ASRK_KV_PAGE * D * 2, p.chunks, done, st);
     }
-    return p.ct == 2 ? launch_shared<D, 2, 4>(c, a, sets * p.chunks, st) : launch_shared<D, 1, 8>(c, a, sets * p.chunks, st);
+    return p.ct == 2 ? launch_shared<D, 2, 4>(c, a, p.chunks, st) : launch_shared<D, 1, 8>(c, a, p.chunks, st);
 }
 
 int check_shape(const asrk_kv_cache* c, int n, int q_heads, int beams) {
     if (int rc = asrk_kv_check(c)) return rc;
     if (n <= 0 || q_heads <= 0 || q_heads % c->kv_heads || beams <= 0 || beams > 32 || c->num_seqs % beams) return ASRK_ERR_SHAPE;
-    if ((int64_t)beams * n * (q_heads / c->kv_heads) > 0x3fffffff) return ASRK_ERR_SHAPE;
+    if ((int64_t)beams * n * (q_heads / c->kv_heads) > 65535 * 128) return ASRK_ERR_SHAPE;  // the grid's last dimension
     return ASRK_OK;
 }
 
@@ -764,8 +779,6 @@ extern "C" int asrk_kv_attention(const asrk_kv_cache* c, int layer, const void* 
     if (layer < 0 || layer >= c->num_layers || seq_ld < 0 || row_ld < 0 || head_ld < 0 || !(scale > 0.f && scale < 1e30f)) return ASRK_ERR_SHAPE;
     if (((uintptr_t)q & 15) || ((uintptr_t)out & 15) || seq_ld % 8 || row_ld % 8 || head_ld % 8) return ASRK_ERR_ALIGN;
     const Plan p = plan_of(c, n, q_heads, num_beams);
-    const int sets = c->num_seqs / num_beams;
-    if ((int64_t)sets * p.chunks * c->kv_heads * p.splits > 0x7fffffff) return ASRK_ERR_SHAPE;
     const int64_t rows = (int64_t)c->num_seqs * n * q_heads;
     AttnArgs a{};
     if (p.splits > 1) {
@@ -786,11 +799,11 @@ extern "C" int asrk_kv_attention(const asrk_kv_cache* c, int layer, const void* 
     a.group = q_heads / c->kv_heads;
     a.beams = num_beams;
     a.splits = p.splits;
-    a.chunks = p.chunks;
-    a.sets = sets;
+    a.per_seq_inv = 1.0 / ((double)n * a.group);
+    a.group_inv = 1.0 / a.group;
     a.c = scale * 1.4426950408889634f;
     hipStream_t st = (hipStream_t)stream;
-    if (int rc = c->head_dim == 64 ? launch_for<64>(c, a, p, sets, st) : launch_for<128>(c, a, p, sets, st)) return rc;
+    if (int rc = c->head_dim == 64 ? launch_for<64>(c, a, p, st) : launch_for<128>(c, a, p, st)) return rc;
     if (p.splits > 1) {
         const int per = 1024 / c->head_dim;
         const dim3 grid((unsigned)((rows + per - 1) / per));

@@ -71,16 +71,6 @@ __device__ __forceinline__ float groups_max(float v) {  // rows of 16 lanes, the
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ int larger(int a, int b) { return a > b ? a : b; }
-__device__ __forceinline__ int wave_imax(int v) {  // v >= 0; shifts within rows of 16, then rows broadcast to later ones
-    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
-    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
-    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
-    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
-    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
-    v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
-    return __builtin_amdgcn_readlane(v, 63);
-}
 __device__ __forceinline__ int over(int x, double inverse) { return (int)(((double)x + 0.5) * inverse); }  // exact
 
 // Grid: x: (head, split), y: set of sequences, z: chunk of columns; whole waves in this order.
@@ -341,7 +331,7 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     Pages work(c, a.beams, set, part * W + wave, a.splits * W);
     Queries<D, CT> qs;
     qs.load(c, cs, first_col, col, g);
-    const int pages = ((wave_imax(qs.most)) + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
+    const int pages = (wave_imax(qs.most) + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
 
     f32x4 o[CT][DT], l[CT];
     float m[CT];
@@ -524,7 +514,7 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
         const int i0 = over(x0, a.group_inv), i1 = over(x1 - 1, a.group_inv) + 1;
         most = i0 >= fresh ? 0 : start + (i1 < fresh ? i1 : fresh);
     } else {
-        most = (wave_imax(held_by));
+        most = wave_imax(held_by);
     }
     int pages = (most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
     pages = pages < c.max_pages ? pages : c.max_pages;
@@ -591,7 +581,7 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
         {
             const float ks = pow2((int8_t)e), vs = pow2(ev - up);
             const int held = (a.beams == 1 ? __builtin_amdgcn_readfirstlane(held_by)
-                                           : (wave_imax((item.with >> lane) & 1 ? held_by : 0))) - item.p * ASRK_KV_PAGE;
+                                           : wave_imax((item.with >> lane) & 1 ? held_by : 0)) - item.p * ASRK_KV_PAGE;
             if (held < ASRK_KV_PAGE) {  // the sequence ends within the page
                 KEEP_BRANCH();
                 const u32x4 mask = keep_before(held, g);

@@ -361,6 +361,11 @@ __device__ __forceinline__ uint32_t to_e4m3x4(float x0, float x1, float x2, floa
         if (!(fabsf(x[i]) < __builtin_inff())) u |= 0x7fu << (8 * i);
     return u;
 }
+// the same of two numbers, already divided
+__device__ __forceinline__ uint32_t to_e4m3x2(float x0, float x1) {
+    const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(__builtin_amdgcn_fmed3f(x0, -448.f, 448.f), __builtin_amdgcn_fmed3f(x1, -448.f, 448.f), 0, false);
+    return w | (fabsf(x0) < __builtin_inff() ? 0u : 0x7fu) | (fabsf(x1) < __builtin_inff() ? 0u : 0x7f00u);
+}
 // four e4m3 bytes times 2^shift (shift <= 0), rounded again
 __device__ __forceinline__ uint32_t shift_e4m3x4(uint32_t u, float factor) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false);
@@ -368,14 +373,83 @@ __device__ __forceinline__ uint32_t shift_e4m3x4(uint32_t u, float factor) {
     return to_e4m3x4(a[0], a[1], b[0], b[1], factor);
 }
 
+// What a page's scales become with new tokens from t0 on, whose largest magnitudes are mk and mv, and the factors of its older ones.
+struct Scales {
+    int ek, ev, flag;
+    float fk = 1.f, fv = 1.f;
+    __device__ __forceinline__ Scales(int old, int t0, float mk, float mv, bool odd) : ek(exponent_of(mk)), ev(exponent_of(mv)), flag(odd) {
+        if (t0 > 0) {
+            const int ok = (int8_t)old, ov = (int8_t)(old >> 8);
+            ek = ek > ok ? ek : ok;
+            ev = ev > ov ? ev : ov;
+            fk = pow2(ok - ek > -60 ? ok - ek : -60);  // 448 2^-60 is zero in e4m3 as well
+            fv = pow2(ov - ev > -60 ? ov - ev : -60);
+            flag |= (old >> 16) & 1;
+        }
+    }
+    __device__ __forceinline__ int word() const { return (ek & 0xff) | ((ev & 0xff) << 8) | (flag << 16); }
+};
+
+// One token: a wave per (head, sequence), a lane per d (D 128: two).  Latency: lengths -> page number -> scales -> stores, and
+// little code; the bytes of the values' column are stored one by one, which needs no read.  320 sequences of 5 heads 5.1 us (the
+// kernel below with one wave, which turns four tokens at a time and reads the others first, 7.5).
+template <class T, int D>
+__global__ __launch_bounds__(64) void kv_write_one_kernel(asrk_kv_cache c, const T* __restrict__ k, const T* __restrict__ v, int64_t seq_ld,
+                                                          int64_t head_ld, int64_t layer) {
+    constexpr int U = D / 64;
+    const int h = blockIdx.x, s = blockIdx.y, lane = threadIdx.x;
+    const int64_t row = (int64_t)s * seq_ld + (int64_t)h * head_ld + lane, slot = (int64_t)s * c.seq_stride;
+    const int start = c.starts[slot], len = c.lens[slot];
+    float kx[U], vx[U], mk = 0.f, mv = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        kx[u] = (float)k[row + 64 * u];
+        vx[u] = (float)v[row + 64 * u];
+    }
+    const int pj = start / ASRK_KV_PAGE, t = start % ASRK_KV_PAGE;
+    if (len <= start || pj >= c.max_pages) return;
+    const int page = c.table[slot * c.max_pages + pj];
+    if (page < 0 || page >= c.num_pages) return;
+    const int64_t at = (layer * c.num_pages + page) * c.kv_heads + h;
+    uint8_t* kp = (uint8_t*)c.kv + at * 2 * ASRK_KV_PAGE * D;
+    uint8_t* vp = kp + ASRK_KV_PAGE * D;
+    int* ep = (int*)c.exps + at;
+    const int old = *ep;
+    bool odd = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        mk = fabsf(kx[u]) < __builtin_inff() ? fmaxf(mk, fabsf(kx[u])) : mk;
+        mv = fabsf(vx[u]) < __builtin_inff() ? fmaxf(mv, fabsf(vx[u])) : mv;
+        odd |= !(fabsf(vx[u]) < __builtin_inff());
+    }
+    const Scales sc(old, t, __uint_as_float(wave_imax(__float_as_uint(mk))), __uint_as_float(wave_imax(__float_as_uint(mv))), __any(odd));
+    if (sc.fk != 1.f)
+        for (int u = lane; u < t * D / 4; u += 64) ((uint32_t*)kp)[u] = shift_e4m3x4(((const uint32_t*)kp)[u], sc.fk);
+    if (sc.fv != 1.f)
+        for (int u = lane; u < D; u += 64)
+            for (int g = 0; g < (t + 3) / 4; ++g) {  // by the lane that stores the new byte of this row, in front of it
+                uint32_t* p = reinterpret_cast<uint32_t*>(vp + u * ASRK_KV_PAGE) + g;
+                *p = shift_e4m3x4(*p, sc.fv);
+            }
+    const float ik = pow2(-sc.ek), iv = pow2(-sc.ev);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int d = lane + 64 * u;
+        const uint32_t two = to_e4m3x2(kx[u] * ik, vx[u] * iv);
+        kp[t * D + d] = (uint8_t)two;
+        vp[d * ASRK_KV_PAGE + t] = (uint8_t)(two >> 8);
+    }
+    if (lane == 0) *ep = sc.word();
+}
+
 // One workgroup per (head, page that new tokens touch, sequence).  The new rows are read once, into registers: the largest
 // magnitude first, then the bytes.  Value bytes are turned through LDS four by four (rows of D + 4 bytes: 16 x 4 lanes read
 // different banks).  Older tokens of the page are only touched if the exponent grows.  Heads vary fastest over the grid:
 // neighbours read, and the rows are whole, together.
-template <class T, int D, int THREADS, int U>  // U pieces of eight values per thread and tensor
-__global__ __launch_bounds__(THREADS) void kv_write_kernel(asrk_kv_cache c, const T* __restrict__ k, const T* __restrict__ v, int64_t seq_ld,
+template <class T, int D>
+__global__ __launch_bounds__(256) void kv_write_kernel(asrk_kv_cache c, const T* __restrict__ k, const T* __restrict__ v, int64_t seq_ld,
                                                            int64_t row_ld, int64_t head_ld, int n, int64_t layer) {
-    constexpr int PER = D / 8, LINE = D + 4;
+    constexpr int THREADS = 256, PER = D / 8, LINE = D + 4, U = ASRK_KV_PAGE * PER / THREADS;  // U pieces of eight values per thread and tensor
     __shared__ __attribute__((aligned(16))) uint8_t turn[ASRK_KV_PAGE * LINE];
     __shared__ uint32_t most[2];
     __shared__ int odd;
@@ -434,18 +508,10 @@ __global__ __launch_bounds__(THREADS) void kv_write_kernel(asrk_kv_cache c, cons
         if (nan_v) atomicOr(&odd, 1);
     }
     __syncthreads();
-    int ek = exponent_of(__uint_as_float(most[0])), ev = exponent_of(__uint_as_float(most[1]));
-    const int ok = (int8_t)old, ov = (int8_t)(old >> 8);
-    float fk = 1.f, fv = 1.f;  // factor of the older tokens
-    if (t0 > 0) {
-        ek = ek > ok ? ek : ok;
-        ev = ev > ov ? ev : ov;
-        fk = pow2(ok - ek > -60 ? ok - ek : -60);  // 448 2^-60 is zero in e4m3 as well
-        fv = pow2(ov - ev > -60 ? ov - ev : -60);
-    }
-    const float ik = pow2(-ek), iv = pow2(-ev);
-    if (t0 > 0 && fk != 1.f)
-        for (int u = threadIdx.x; u < t0 * D / 4; u += THREADS) ((uint32_t*)kp)[u] = shift_e4m3x4(((const uint32_t*)kp)[u], fk);
+    const Scales sc(old, t0, __uint_as_float(most[0]), __uint_as_float(most[1]), odd);
+    const float ik = pow2(-sc.ek), iv = pow2(-sc.ev);
+    if (sc.fk != 1.f)
+        for (int u = threadIdx.x; u < t0 * D / 4; u += THREADS) ((uint32_t*)kp)[u] = shift_e4m3x4(((const uint32_t*)kp)[u], sc.fk);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
         const int u = j * THREADS + threadIdx.x;
@@ -462,7 +528,7 @@ __global__ __launch_bounds__(THREADS) void kv_write_kernel(asrk_kv_cache c, cons
     }
     __syncthreads();
     // four tokens by four d's per step; lanes run over the tokens first, so that stores are whole lines
-    const bool shift = t0 > 0 && fv != 1.f;
+    const bool shift = sc.fv != 1.f;
     const int g0 = shift ? 0 : t0 / 4, gs = (t1 + 3) / 4 - g0;
     for (int u = threadIdx.x; u < gs * (D / 4); u += THREADS) {
         const int g = g0 + u % gs, d = u / gs * 4;
@@ -483,27 +549,24 @@ __global__ __launch_bounds__(THREADS) void kv_write_kernel(asrk_kv_cache c, cons
             uint32_t* p = reinterpret_cast<uint32_t*>(vp + (d + i) * ASRK_KV_PAGE + g * 4);
             if (mask != 0xffffffffu) {
                 uint32_t o = *p;
-                if (shift) o = shift_e4m3x4(o, fv);
+                if (shift) o = shift_e4m3x4(o, sc.fv);
                 x[i] = (x[i] & mask) | (o & ~mask);
             }
             *p = x[i];
         }
     }
-    if (threadIdx.x == 0) {
-        const int flag = odd | (t0 > 0 ? (old >> 16) & 1 : 0);
-        *reinterpret_cast<int*>(ep) = (ek & 0xff) | ((ev & 0xff) << 8) | (flag << 16);
-    }
+    if (threadIdx.x == 0) *reinterpret_cast<int*>(ep) = sc.word();
 }
 template <class T, int D>
 void launch_write(const asrk_kv_cache* c, const void* k, const void* v, int64_t seq_ld, int64_t row_ld, int64_t head_ld, int n, int layer,
                   hipStream_t st) {
+    if (n == 1) {
+        hipLaunchKernelGGL((kv_write_one_kernel<T, D>), dim3(c->kv_heads, c->num_seqs), dim3(64), 0, st, *c, (const T*)k, (const T*)v, seq_ld,
+                           head_ld, (int64_t)layer);
+        return;
+    }
     const dim3 grid(c->kv_heads, (unsigned)(((int64_t)n + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1), c->num_seqs);
-    if (n == 1)  // D / 8 pieces of work: one wave
-        hipLaunchKernelGGL((kv_write_kernel<T, D, 64, 1>), grid, dim3(64), 0, st, *c, (const T*)k, (const T*)v, seq_ld, row_ld, head_ld, n,
-                           (int64_t)layer);
-    else
-        hipLaunchKernelGGL((kv_write_kernel<T, D, 256, D / 32>), grid, dim3(256), 0, st, *c, (const T*)k, (const T*)v, seq_ld, row_ld,
-                           head_ld, n, (int64_t)layer);
+    hipLaunchKernelGGL((kv_write_kernel<T, D>), grid, dim3(256), 0, st, *c, (const T*)k, (const T*)v, seq_ld, row_ld, head_ld, n, (int64_t)layer);
 }
 
 // ---- tokens out

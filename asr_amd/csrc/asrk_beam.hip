@@ -5,8 +5,9 @@
 // and the best n = 2 K of the K V values, ties to the lowest k V + v.  A beam whose score or largest logit is not
 // finite, or that holds a NaN, offers -inf throughout.
 //
-// HBM-bound where it is large (32 x 8 beams, 128001 fp32 words, 131 MB: chunk kernel 27.5 us = 4.8 TB/s, join 10; 64 x 5,
-// 51865 bf16 words, 33 MB: 14.2 and 7, bound by instructions and latency): every logit is read once, into registers.  Rows are cut into chunks of 8192 so that one utterance already
+// HBM-bound where it is large (32 x 8 beams, 128001 fp32 words, 131 MB: chunk kernel 25.9 us = 5.1 TB/s, join 8.6; 64 x 5,
+// 51865 bf16 words, 33 MB: 13.9 and 5.7, bound by instructions and latency): every logit is read once, into registers.  Rows
+// are cut into chunks of 8192 so that one utterance already
 // gives 7 workgroups per beam at 50 k words; a second, small launch joins the chunks.  (One launch with a last-block
 // counter would need that counter cleared, and shared, between calls; two launches need neither.)
 #include "asrk_common.h"
@@ -37,6 +38,10 @@ template <>
 struct SelVec<float> {
     typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(4)));
     static constexpr int N = 4;
+    static __device__ __forceinline__ u32x4 place(float v, int i) {
+        const uint32_t w = __float_as_uint(v);
+        return u32x4{i == 0 ? w : 0, i == 1 ? w : 0, i == 2 ? w : 0, i == 3 ? w : 0};
+    }
     static __device__ __forceinline__ void unpack(u32x4 r, float* x) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r[i]);
@@ -46,6 +51,10 @@ template <>
 struct SelVec<bf16_t> {
     typedef uint32_t Raw __attribute__((ext_vector_type(4), aligned(2)));
     static constexpr int N = 8;
+    static __device__ __forceinline__ u32x4 place(bf16_t v, int i) {
+        const uint32_t w = (__float_as_uint((float)v) >> 16) << (16 * (i & 1));
+        return u32x4{i / 2 == 0 ? w : 0, i / 2 == 1 ? w : 0, i / 2 == 2 ? w : 0, i / 2 == 3 ? w : 0};
+    }
     static __device__ __forceinline__ void unpack(u32x4 r, float* x) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -54,6 +63,24 @@ struct SelVec<bf16_t> {
         }
     }
 };
+
+// Maximum and sum over a wave: shifts within rows of 16, then rows broadcast to later ones.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ float from_lane(float v, float none) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(__float_as_uint(none), __float_as_uint(v), CONTROL, ROWS, 0xf, false));
+}
+template <class F>
+__device__ __forceinline__ float over_wave(float v, float none, F&& f) {
+    v = f(v, from_lane<0x111, 0xf>(v, none));
+    v = f(v, from_lane<0x112, 0xf>(v, none));
+    v = f(v, from_lane<0x114, 0xf>(v, none));
+    v = f(v, from_lane<0x118, 0xf>(v, none));
+    v = f(v, from_lane<0x142, 0xa>(v, none));
+    v = f(v, from_lane<0x143, 0xc>(v, none));
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+}
+__device__ __forceinline__ float sel_max(float v) { return over_wave(v, NEG_INF, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float sel_sum(float v) { return over_wave(v, 0.f, [](float a, float b) { return a + b; }); }
 
 constexpr int sel_lanes(int n) { return n + 8; }  // lanes of a workgroup whose values may be candidates
 
@@ -74,22 +101,35 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ l
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = blockIdx.y, chunk = blockIdx.x;
     const T* p = logits + (int64_t)row * ld;
-    const int e0 = (chunk * SEL_WAVES + wave) * 64 * SEL_EPT + lane * VEC;  // word of slot 0; slot s: word(s), ascending
-    auto word = [&](int s) __attribute__((always_inline)) { return e0 + s / VEC * 64 * VEC + s % VEC; };
+    const int e0 = (chunk * SEL_WAVES + wave) * 64 * SEL_EPT + lane * VEC;  // word of slot 0
+    // A piece that passes the row's end is taken so that it ends there; what it then has in common with the piece in front, and
+    // all of the pieces behind, is masked.
+    const int last = V - VEC;
+    auto nominal = [&](int s) __attribute__((always_inline)) { return e0 + s / VEC * 64 * VEC; };
+    auto begin = [&](int s) __attribute__((always_inline)) { return nominal(s) < last ? nominal(s) : last; };
+    auto word = [&](int s) __attribute__((always_inline)) { return begin(s) + s % VEC; };  // ascending
+    auto real = [&](int s) __attribute__((always_inline)) { return s % VEC >= nominal(s) - begin(s); };
     float x[SEL_EPT];
-    if (e0 + (SEL_EPT / VEC - 1) * 64 * VEC + VEC <= V) {
+    const int first_word = __builtin_amdgcn_readfirstlane(e0);
+    if (first_word >= V) {
 #pragma unroll
-        for (int j = 0; j < SEL_EPT / VEC; ++j)
-            SelVec<T>::unpack(*reinterpret_cast<const typename SelVec<T>::Raw*>(p + word(j * VEC)), x + j * VEC);
+        for (int s = 0; s < SEL_EPT; ++s) x[s] = NEG_INF;
     } else {
+        u32x4 raw[SEL_EPT / VEC];
+        if (V >= VEC) {
 #pragma unroll
-        for (int j = 0; j < SEL_EPT / VEC; ++j) {
-            if (word(j * VEC) + VEC <= V) {
-                SelVec<T>::unpack(*reinterpret_cast<const typename SelVec<T>::Raw*>(p + word(j * VEC)), x + j * VEC);
-            } else {
+            for (int j = 0; j < SEL_EPT / VEC; ++j) raw[j] = *reinterpret_cast<const typename SelVec<T>::Raw*>(p + begin(j * VEC));
+        } else {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) x[j * VEC + i] = word(j * VEC + i) < V ? (float)p[word(j * VEC + i)] : NEG_INF;
-            }
+            for (int j = 0; j < SEL_EPT / VEC; ++j) raw[j] = u32x4{0, 0, 0, 0};
+            for (int i = 0; i < V; ++i) raw[0] |= SelVec<T>::place(p[i], i - last);
+        }
+#pragma unroll
+        for (int j = 0; j < SEL_EPT / VEC; ++j) SelVec<T>::unpack(raw[j], x + j * VEC);
+        if (first_word + 64 * SEL_EPT > V) {
+            asm volatile("");  // a branch: masks cost whole waves as much as the maximum does
+#pragma unroll
+            for (int s = 0; s < SEL_EPT; ++s) x[s] = real(s) ? x[s] : NEG_INF;
         }
     }
     float best = NEG_INF;
@@ -98,12 +138,12 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ l
     // the lane maxima of all four waves, lane l of wave w at 4 l + w; 0: no word at all
     bests[lane * 4 + wave] = e0 < V ? ord32(best + 0.0f) : 0;  // -0 counts as 0
     if (threadIdx.x == 0) count = 0;
-    const float top = wave_max(best);
+    const float top = sel_max(best);
     const float ref = top > NEG_INF ? top : 0.f;
     float sum = 0.f;  // NaN if one of the logits is
 #pragma unroll
     for (int s = 0; s < SEL_EPT; ++s) sum += __builtin_amdgcn_exp2f((x[s] - ref) * 1.4426950408889634f);
-    sum = wave_sum(sum);
+    sum = sel_sum(sum);
     if (lane == 0)
         stats[((int64_t)row * gridDim.x + chunk) * SEL_WAVES + wave] = make_float2(sum == sum ? top : __builtin_inff(), sum);
     __syncthreads();
@@ -121,7 +161,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ l
         uint32_t lo = LOWEST, hi = 0xff800001u;  // at or above lo: too many; hi: too few (above +inf)
         bool found = false;
         {  // most lane maxima lie within a few units below the largest
-            float m = wave_max(fmaxf(fmaxf(unord32(mine[0] ? mine[0] : LOWEST), unord32(mine[1] ? mine[1] : LOWEST)),
+            float m = sel_max(fmaxf(fmaxf(unord32(mine[0] ? mine[0] : LOWEST), unord32(mine[1] ? mine[1] : LOWEST)),
                                      fmaxf(unord32(mine[2] ? mine[2] : LOWEST), unord32(mine[3] ? mine[3] : LOWEST))));
             hi = __builtin_amdgcn_readfirstlane(ord32(m)) + 1;
         }
@@ -136,7 +176,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ l
         if (!found) {  // the n-th lane by (value, ~word)
             uint32_t first = 0;
 #pragma unroll
-            for (int s = SEL_EPT - 1; s >= 0; --s) first = x[s] == best ? 0xffffffffu - (uint32_t)word(s) : first;
+            for (int s = SEL_EPT - 1; s >= 0; --s) first = x[s] == best && real(s) ? 0xffffffffu - (uint32_t)word(s) : first;
             firsts[lane * 4 + wave] = first;
             __syncthreads();  // every wave is here: they all look at the same 256 values
             for (int w = 0; w < 4; ++w) {
@@ -158,7 +198,7 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ l
         for (int s = 0; s < SEL_EPT; ++s) {
             if (!__any(x[s] >= least)) continue;
             const uint32_t high = ord32(x[s] + 0.0f), low = 0xffffffffu - (uint32_t)word(s);
-            if (x[s] >= least && word(s) < V && (high > tau || low >= tau_low)) cand[atomicAdd(&count, 1)] = ((uint64_t)high << 32) | low;
+            if (x[s] >= least && real(s) && (high > tau || low >= tau_low)) cand[atomicAdd(&count, 1)] = ((uint64_t)high << 32) | low;
         }
     }
     __syncthreads();
@@ -169,8 +209,9 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ l
     for (int t = threadIdx.x >> 2; t < (total + 63) / 64 * 64; t += 64) {
         const uint64_t key = t < total ? cand[t] : 0;
         int r = 0;
-#pragma unroll 4
-        for (int u = part; u < total; u += 4) r += cand[u] > key ? 1 : 0;
+        for (int u0 = part; u0 < total; u0 += 16)
+#pragma unroll
+            for (int u = u0; u < u0 + 16; u += 4) r += (u < total) & (cand[u < total ? u : 0] > key);
         r += __shfl_xor(r, 1, 64);
         r += __shfl_xor(r, 2, 64);
         if (part == 0 && t < total && r < n) out[r] = key;
@@ -181,7 +222,7 @@ struct Pick {
     double v;
     uint32_t at;
 };
-__device__ __forceinline__ bool ahead(const Pick& a, const Pick& b) { return a.v > b.v || (a.v == b.v && a.at < b.at); }
+__device__ __forceinline__ bool ahead(const Pick& a, const Pick& b) { return (a.v > b.v) | ((a.v == b.v) & (a.at < b.at)); }
 
 // One workgroup per utterance: the row sums in 64 bits, then the best n of the chunks' sorted lists.  Values are
 // compared in 64 bits, where different logits of a beam stay different (and equal ones equal); the n-th best list head
@@ -189,12 +230,21 @@ __device__ __forceinline__ bool ahead(const Pick& a, const Pick& b) { return a.v
 // dependent steps: everything it may need is loaded first (a load is about a microsecond, the arithmetic is less).
 constexpr int JOIN_T = 512;
 constexpr int JOIN_HELD = 4;  // keys per thread that are loaded ahead: all of them up to 2048
+__device__ __forceinline__ int over(int x, float inverse) { return (int)(((float)x + 0.5f) * inverse); }  // exact: x < 2^16, divisors up to 2048
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ double from_lane(double v) {  // 0 where there is none
+    const uint64_t b = __double_as_longlong(v);
+    const uint32_t low = __builtin_amdgcn_update_dpp(0, (uint32_t)b, CONTROL, ROWS, 0xf, false);
+    const uint32_t high = __builtin_amdgcn_update_dpp(0, (uint32_t)(b >> 32), CONTROL, ROWS, 0xf, false);
+    return __longlong_as_double((int64_t)(((uint64_t)high << 32) | low));
+}
 __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __restrict__ keys, const float2* __restrict__ stats,
                                                            const float* __restrict__ scores, int K, int V, int chunks, int n,
                                                            int64_t eos, float* __restrict__ out_scores,
                                                            int64_t* __restrict__ out_tokens, int64_t* __restrict__ out_parents,
                                                            float* __restrict__ cand_scores, int64_t* __restrict__ cand_tokens,
                                                            int64_t* __restrict__ cand_parents) {
+    __shared__ uint64_t ahead_keys[JOIN_HELD * JOIN_T];
     __shared__ double lse[SEL_MAX_BEAMS];
     __shared__ double score[SEL_MAX_BEAMS];
     __shared__ int alive[SEL_MAX_BEAMS];
@@ -226,26 +276,33 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
         const float2 first = lane < chunks * SEL_WAVES ? st[lane] : make_float2(NEG_INF, 0.f);
         float top = first.x;
         for (int i = lane + 64; i < chunks * SEL_WAVES; i += 64) top = fmaxf(top, st[i].x);
-        top = wave_max(top);
+        top = sel_max(top);
         const bool ok = top > NEG_INF && top < __builtin_inff();
         double sum = 0.0;
-        if (ok) {
-            if (first.x > NEG_INF) sum = (double)first.y * exp((double)first.x - (double)top);
-            for (int i = lane + 64; i < chunks * SEL_WAVES; i += 64)
-                if (st[i].x > NEG_INF) sum += (double)st[i].y * exp((double)st[i].x - (double)top);
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        if (lane == 0) {
+        if (ok)
+            for (int i = lane; i < chunks * SEL_WAVES; i += 64) {
+                const float2 one = i == lane ? first : st[i];
+                if (one.x > NEG_INF) sum += (double)one.y * exp((double)one.x - (double)top);
+            }
+        sum += from_lane<0x111, 0xf>(sum);
+        sum += from_lane<0x112, 0xf>(sum);
+        sum += from_lane<0x114, 0xf>(sum);
+        sum += from_lane<0x118, 0xf>(sum);
+        sum += from_lane<0x142, 0xa>(sum);
+        sum += from_lane<0x143, 0xc>(sum);
+        if (lane == 63) {
             alive[k] = ok && s > NEG_INF && s < __builtin_inff();
             lse[k] = ok ? (double)top + log(sum) : 0.0;
             score[k] = (double)s;
         }
     }
+#pragma unroll
+    for (int q = 0; q < JOIN_HELD; ++q) ahead_keys[q * JOIN_T + threadIdx.x] = held[q];
     __syncthreads();
+    const float n_inv = 1.f / (float)n, chunks_inv = 1.f / (float)chunks;
     // entry j of list l, whose key is `key`; false: none
     auto entry = [&](int l, int j, uint64_t key, Pick& p) -> bool {
-        const int k = l / chunks;
+        const int k = over(l, chunks_inv);
         if (!alive[k]) {  // a dead beam: its words in order
             p = Pick{-__builtin_inf(), (uint32_t)(k * V + j)};
             return l == k * chunks && j < V;
@@ -254,12 +311,10 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
         return key != 0;
     };
     auto each = [&](auto&& f) __attribute__((always_inline)) {  // f(list, place in it, key)
-#pragma unroll
-        for (int q = 0; q < JOIN_HELD; ++q) {
-            const int i = q * JOIN_T + threadIdx.x;
-            if (i < all) f(i / n, i % n, held[q]);
+        for (int i = threadIdx.x; i < all; i += JOIN_T) {
+            const int l = over(i, n_inv);
+            f(l, i - l * n, i < JOIN_HELD * JOIN_T ? ahead_keys[i] : mine[i]);
         }
-        for (int i = JOIN_HELD * JOIN_T + threadIdx.x; i < all; i += JOIN_T) f(i / n, i % n, mine[i]);
     };
     each([&](int l, int j, uint64_t key) {
         if (j) return;
@@ -273,8 +328,9 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
     for (int l = threadIdx.x >> 2; l < lists; l += JOIN_T / 4) {
         const Pick p{head_v[l], head_at[l]};
         int r = 0;
-#pragma unroll 4
-        for (int u = part; u < lists; u += 4) r += ahead(Pick{head_v[u], head_at[u]}, p) ? 1 : 0;  // NaN is ahead of nothing
+        for (int u0 = part; u0 < lists; u0 += 16)
+#pragma unroll
+            for (int u = u0; u < u0 + 16; u += 4) r += (u < lists) & ahead(Pick{head_v[u], head_at[u]}, p);  // NaN is ahead of nothing
         r += __shfl_xor(r, 1, 64);
         r += __shfl_xor(r, 2, 64);
         if (part == 0 && r == n - 1 && p.v == p.v) tau = p;
@@ -294,8 +350,9 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
     for (int t = threadIdx.x >> 2; t < c; t += JOIN_T / 4) {
         const Pick p{cand_v[t], cand_at[t]};
         int r = 0;
-#pragma unroll 4
-        for (int u = part; u < c; u += 4) r += ahead(Pick{cand_v[u], cand_at[u]}, p) ? 1 : 0;
+        for (int u0 = part; u0 < c; u0 += 16)
+#pragma unroll
+            for (int u = u0; u < u0 + 16; u += 4) r += (u < c) & ahead(Pick{cand_v[u], cand_at[u]}, p);
         r += __shfl_xor(r, 1, 64);
         r += __shfl_xor(r, 2, 64);
         if (part == 0 && r < n) {

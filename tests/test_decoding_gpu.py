@@ -60,6 +60,20 @@ def test_select(B, K, V, dtype, pad):
         check_select(x.view(B, K, V), s, eos=0)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [2, 2050])
+def test_select_rows_that_end_anywhere(rows, dtype):
+    """Rows that end within a piece, a wave's share or a chunk, with NaN behind them."""
+    g = _gen(rows)
+    sizes = [*range(2, 19), 255, 256, 257, 511, 513, 2047, 2051, 4100, 8190, 8191, 8195, 8199, 8200, 16383, 16385, 16391]
+    for V in sizes if rows == 2 else (3, 9, 513, 8191, 8199, 8200):
+        x = (torch.randn((rows, V + 9), generator=g, device="cuda") * 3).to(torch.bfloat16 if dtype == "bf16" else torch.float32)
+        x[:, V:] = math.nan
+        s = -torch.rand((rows // 2, 2), generator=g, device="cuda")
+        check_select(x[:, :V], s)
+        check_select(x.view(-1)[1:1 + rows // 2 * 2 * (V + 8)].view(rows, V + 8)[:, :V].nan_to_num(0.25).contiguous(), s, eos=1)
+
+
 def test_select_last_position_of_a_run():
     x = torch.randn((6, 4, 1001), generator=_gen(5), device="cuda")
     check_select(x[:, -1], -torch.rand((2, 3), generator=_gen(6), device="cuda"))

@@ -571,18 +571,25 @@ void launch_write(const asrk_kv_cache* c, const void* k, const void* v, int64_t 
 
 // ---- tokens out
 
-// One workgroup per (page, head, layer and sequence) of the tokens [first, first + count) of every sequence.  The value
-// page is turned through LDS (rows of 68 bytes: 8 x 8 lanes read different banks).  HBM-bound: 25600 pages (629 MB) 142 us =
-// 4.4 TB/s; with the heads slowest over the grid, whose lines of a row are then written far apart in time, 192.
+// One workgroup per (page, head, layer and sequence) of the tokens [first, first + count) of every sequence.  Both pages are
+// loaded at once; the value page is turned through LDS (rows of 68 bytes: 8 x 8 lanes read different banks), two tokens of eight d's
+// per step.  HBM-bound: 25600 pages (629 MB) 120 us = 5.2 TB/s; with the heads slowest over the grid, whose lines of a row are then
+// written far apart in time, a third more.
+template <int D>
 __global__ __launch_bounds__(256) void kv_read_kernel(asrk_kv_cache c, const int* __restrict__ first_each, int first_all, int count,
                                                       int layer0, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out) {
-    __shared__ uint32_t turn[128 * 17];
-    const int D = c.head_dim, H = c.kv_heads, M = c.max_pages;
+    constexpr int PER = D / 8, UK = ASRK_KV_PAGE * PER / 256, UV = D * ASRK_KV_PAGE / 16 / 256;
+    __shared__ uint32_t turn[D * 17];
+    const int H = c.kv_heads, M = c.max_pages;
     const int h = blockIdx.x;
-    const int s = blockIdx.z % c.num_seqs, l = blockIdx.z / c.num_seqs;
+    int s = blockIdx.z, l = 0;
+    if ((int)gridDim.z != c.num_seqs) {
+        l = (unsigned)s / (unsigned)c.num_seqs;
+        s -= l * c.num_seqs;
+    }
     const int64_t slot = (int64_t)s * c.seq_stride;
     const int64_t first = first_each ? first_each[s] : first_all;
-    const int64_t pj = (first < 0 ? -((-first + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE) : first / ASRK_KV_PAGE) + blockIdx.y;
+    const int64_t pj = (first >> 6) + blockIdx.y;  // pages of 64, also of what lies in front of the sequence
     const int64_t t_lo = first - pj * ASRK_KV_PAGE, t_hi = first + count - pj * ASRK_KV_PAGE;  // asked tokens within the page
     if (t_hi <= 0) return;
     const int lo = t_lo > 0 ? (int)t_lo : 0, hi = t_hi < ASRK_KV_PAGE ? (int)t_hi : ASRK_KV_PAGE;
@@ -597,52 +604,52 @@ __global__ __launch_bounds__(256) void kv_read_kernel(asrk_kv_cache c, const int
     const uint8_t* kp = (const uint8_t*)c.kv + at * 2 * ASRK_KV_PAGE * D;
     const uint8_t* vp = kp + ASRK_KV_PAGE * D;
     const int e = *reinterpret_cast<const int*>(c.exps + at * 4);
+    u32x2 kx[UK];
+    u32x4 vx[UV];
+    if (have) {
+#pragma unroll
+        for (int j = 0; j < UV; ++j) vx[j] = reinterpret_cast<const u32x4*>(vp)[j * 256 + threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < UK; ++j) kx[j] = reinterpret_cast<const u32x2*>(kp)[j * 256 + threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < UV; ++j) {
+            const int u = j * 256 + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) turn[(u >> 2) * 17 + (u & 3) * 4 + i] = vx[j][i];
+        }
+    }
+    __syncthreads();
     const float sk = pow2((int8_t)e), sv = pow2((int8_t)(e >> 8));
     const int64_t out0 = (((int64_t)l * c.num_seqs + s) * count - t_lo) * H * D + (int64_t)h * D;  // of token 0 of the page
-    const int per = D / 8;
-    if (have)
-        for (int u = threadIdx.x; u < D * 16; u += 256) turn[(u / 16) * 17 + u % 16] = ((const uint32_t*)vp)[u];
-    __syncthreads();
-    for (int u = threadIdx.x; u < (hi - lo) * per; u += 256) {
-        const int t = lo + u / per, d = (u % per) * 8;
-        bf16x8 y;
+#pragma unroll
+    for (int j = 0; j < UK; ++j) {
+        const int u = j * 256 + threadIdx.x, t = u / PER, d = u % PER * 8;
+        if (t < lo || t >= hi) continue;
+        u32x4 y = {0, 0, 0, 0};
         if (t < have) {
-            const u32x2 w = *reinterpret_cast<const u32x2*>(kp + t * D + d);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], sk, false);
-                const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], sk, true);
-                y[4 * i] = a[0]; y[4 * i + 1] = a[1]; y[4 * i + 2] = b[0]; y[4 * i + 3] = b[1];
+                y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kx[j][i], sk, false));
+                y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(kx[j][i], sk, true));
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = (bf16_t)0.f;
         }
-        *reinterpret_cast<bf16x8*>(k_out + out0 + (int64_t)t * H * D + d) = y;
+        *reinterpret_cast<u32x4*>(k_out + out0 + (int64_t)t * H * D + d) = y;
     }
-    for (int u = threadIdx.x; u < 16 * per; u += 256) {  // four tokens, eight d
-        const int g = u / per, d = (u % per) * 8;
-        if (g * 4 >= hi || g * 4 + 4 <= lo) continue;
-        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = have ? turn[(d + i) * 17 + g] : 0;
+    for (int j = 0; j < UK / 2; ++j) {
+        const int u = j * 256 + threadIdx.x, t = u / PER * 2, d = u % PER * 8;
+        uint32_t two[8];  // tokens t and t + 1 of d + i
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int t = g * 4 + j;
-            if (t < lo || t >= hi) continue;
-            bf16x8 y;
+        for (int i = 0; i < 8; ++i)
+            two[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(turn[(d + i) * 17 + t / 4] >> (8 * (t & 2)), sv, false));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = (bf16_t)0.f;
-            if (t < have) {
+        for (int o = 0; o < 2; ++o) {
+            if (t + o < lo || t + o >= hi) continue;
+            u32x4 y = {0, 0, 0, 0};
+            if (t + o < have)
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const uint32_t two = ((w[i] >> (8 * j)) & 0xffu) | (((w[i + 1] >> (8 * j)) & 0xffu) << 8);
-                    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, sv, false);
-                    y[i] = a[0];
-                    y[i + 1] = a[1];
-                }
-            }
-            *reinterpret_cast<bf16x8*>(v_out + out0 + (int64_t)t * H * D + d) = y;
+                for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_perm(two[2 * i + 1], two[2 * i], o ? 0x07060302 : 0x05040100);
+            *reinterpret_cast<u32x4*>(v_out + out0 + (int64_t)(t + o) * H * D + d) = y;
         }
     }
 }
@@ -734,7 +741,7 @@ extern "C" int asrk_kv_read(const asrk_kv_cache* c, int layer, int layers, const
     const int64_t parts = ((int64_t)count + ASRK_KV_PAGE - 2) / ASRK_KV_PAGE + 1;  // pages that `count` tokens can touch
     if (parts > 65535) return ASRK_ERR_SHAPE;
     const dim3 grid(c->kv_heads, (unsigned)parts, c->num_seqs * layers);
-    hipLaunchKernelGGL(kv_read_kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, first_each, first_all, count, layer, (bf16_t*)k_out,
-                       (bf16_t*)v_out);
+    auto* const kernel = c->head_dim == 64 ? kv_read_kernel<64> : kv_read_kernel<128>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, *c, first_each, first_all, count, layer, (bf16_t*)k_out, (bf16_t*)v_out);
     return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
 }

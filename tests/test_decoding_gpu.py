@@ -216,6 +216,25 @@ def test_write_is_right_at_the_ends_of_the_range():
         same_tokens(c, o, 0, 70)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("where", ["keys", "values", "both"])
+def test_write_bf16_at_the_ends_of_the_range(dim, where):
+    """Pages with and without numbers that are not finite or saturate, in the keys, the values or both."""
+    g = _gen(dim)
+    c, o = both(3, 200, 2, dim)
+    for n in (1, 70, 1, 5, 64):
+        k, v = (torch.randn((3, n, 2, dim), generator=g, device="cuda").bfloat16() for _ in range(2))
+        for x in {"keys": [k], "values": [v], "both": [k, v]}[where]:
+            x[0, n // 2, 0, 3:7] = torch.tensor([math.inf, -math.inf, math.nan, -3e38], device="cuda").bfloat16()
+            x[1, n - 1, 1, :2] = torch.tensor([3.3e38, -2.0 ** 127], device="cuda").bfloat16()
+            x[2, 0, 0, dim - 1] = -math.nan
+        c.extend(n)
+        o.extend(n)
+        c.write(k, v)
+        o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+        same_tokens(c, o, 0, 200)
+
+
 def test_write_takes_any_strides():
     c, o = both(2, 130, 2, 64)
     g = _gen(8)

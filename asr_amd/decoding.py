@@ -18,7 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import NamedTuple, Optional, Tuple, Union
+from typing import Dict, List, NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -207,6 +207,7 @@ class PagedKVCache:
         self._c = _lib.KVCache(self.num_layers, self.num_pages, self.kv_heads, self.head_dim, self.num_seqs, self.max_len // PAGE,
                                self._seq_stride, *[ctypes.c_void_p(t.data_ptr()) for t in ptrs])
         self._ref = ctypes.byref(self._c)
+        self._workspace: Dict[Tuple[int, int, int], int] = {}  # bytes that attend needs, by new tokens, heads and beams
 
     def leaders(self, num_beams: int) -> "PagedKVCache":
         """A view of every ``num_beams``-th sequence (beam 0 of each utterance), on the same pages."""
@@ -276,35 +277,38 @@ class PagedKVCache:
         return layer
 
     @staticmethod
-    def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
+    def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, List[int]]:
         """x [S, n, heads, dim] with dense last dimension and rows at 16 bytes, and its other strides."""
-        per = 16 // x.element_size()
-        lds = tuple(0 if size == 1 else st for size, st in zip(x.shape[:3], x.stride()))
-        if x.stride(3) != 1 or any(st % per for st in lds) or x.data_ptr() % 16:
-            x = x.clone(memory_format=torch.contiguous_format)
-            lds = tuple(x.stride()[:3])
+        mask = 16 // x.element_size() - 1
+        *lds, one = x.stride()
+        if one != 1 or (lds[0] | lds[1] | lds[2]) & mask or x.data_ptr() & 15:  # a dimension of size 1 may have any stride
+            lds = [0 if size == 1 else st for size, st in zip(x.shape, lds)]
+            if one != 1 or (lds[0] | lds[1] | lds[2]) & mask or x.data_ptr() & 15:
+                x = x.clone(memory_format=torch.contiguous_format)
+                lds = list(x.stride()[:3])
         return x, lds
 
     def write(self, k: torch.Tensor, v: torch.Tensor, layer: int = 0) -> None:
         """The new tokens' keys and values of one layer: ``k``, ``v`` [num_seqs, n, kv_heads, head_dim] (float32 or bfloat16, any
         strides).  Row i of sequence s is its token ``starts[s] + i``; rows behind ``lens[s]`` are not looked at, and new tokens
         that no row is given for are not written."""
-        shape = (self.num_seqs, self.kv_heads, self.head_dim)
-        if k.dim() != 4 or k.shape != v.shape or (k.shape[0], *k.shape[2:]) != shape:
-            raise ValueError(f"k and v must be [{shape[0]}, n, {shape[1]}, {shape[2]}], got {list(k.shape)} and {list(v.shape)}")
+        shape = k.shape
+        if len(shape) != 4 or shape != v.shape or shape[0] != self.num_seqs or shape[2] != self.kv_heads or shape[3] != self.head_dim:
+            raise ValueError(f"k and v must be [{self.num_seqs}, n, {self.kv_heads}, {self.head_dim}], got {list(shape)} and {list(v.shape)}")
         if k.dtype not in _DT or v.dtype != k.dtype:
             raise ValueError("k and v must both be float32 or bfloat16")
         self._mine("write", k, v)
         layer = self._layer(layer)
-        if k.shape[1] == 0:
+        n = shape[1]
+        if n == 0:
             return
-        if k.shape[1] > 65534 * PAGE:
-            raise ValueError(f"cannot write {k.shape[1]} tokens in one call")
+        if n > 65534 * PAGE:
+            raise ValueError(f"cannot write {n} tokens in one call")
         (k, lds), (v, v_lds) = self._rows(k), self._rows(v)
         if lds != v_lds:
             k, v = k.contiguous(), v.contiguous()
-            lds = tuple(k.stride()[:3])
-        _call("asrk_kv_write", self.device, self._ref, layer, k.data_ptr(), v.data_ptr(), _DT[k.dtype], *lds, k.shape[1])
+            lds = k.stride()[:3]
+        _call("asrk_kv_write", self.device, self._ref, layer, k.data_ptr(), v.data_ptr(), _DT[k.dtype], *lds, n)
 
     def read(self, first: Union[int, torch.Tensor], count: int, layer: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Tokens ``first`` .. ``first + count - 1`` of every sequence (an int, or an integer [num_seqs] tensor) as they are
@@ -337,8 +341,9 @@ class PagedKVCache:
 
         ``num_beams`` consecutive sequences are worked on together, and pages that they share are read once.  It changes
         no result but for rounding: the beams may share any pages, or none."""
-        if q.dim() != 4 or q.shape[0] != self.num_seqs or q.shape[3] != self.head_dim or q.shape[2] < 1 or q.shape[2] % self.kv_heads:
-            raise ValueError(f"q must be [{self.num_seqs}, n, a multiple of {self.kv_heads}, {self.head_dim}], got {list(q.shape)}")
+        shape = q.shape
+        if len(shape) != 4 or shape[0] != self.num_seqs or shape[3] != self.head_dim or shape[2] < 1 or shape[2] % self.kv_heads:
+            raise ValueError(f"q must be [{self.num_seqs}, n, a multiple of {self.kv_heads}, {self.head_dim}], got {list(shape)}")
         if q.dtype != torch.bfloat16:
             raise ValueError("q must be bfloat16")
         if not 1 <= num_beams <= 32 or self.num_seqs % num_beams:
@@ -348,12 +353,16 @@ class PagedKVCache:
             raise ValueError(f"scale must be positive, got {scale}")
         self._mine("attend", q)
         layer = self._layer(layer)
-        out = q.new_empty(q.shape)
-        if out.numel() == 0:
+        n, heads = shape[1], shape[2]
+        if num_beams * n * (heads // self.kv_heads) > 65535 * 128:
+            raise ValueError(f"cannot attend {n} tokens of {num_beams} beams in one call")
+        out = q.new_empty(shape)
+        if n == 0:
             return out
         q, lds = self._rows(q)
-        n, heads = q.shape[1], q.shape[2]
-        need = _lib.load().asrk_kv_attention_workspace_bytes(self._ref, n, heads, num_beams)
+        need = self._workspace.get((n, heads, num_beams))
+        if need is None:
+            need = self._workspace[n, heads, num_beams] = _lib.load().asrk_kv_attention_workspace_bytes(self._ref, n, heads, num_beams)
         ws = q.new_empty((need,), dtype=torch.uint8) if need else None
         _call("asrk_kv_attention", self.device, self._ref, layer, q.data_ptr(), *lds, n, heads, num_beams, scale, out.data_ptr(), _address(ws), need)
         return out

@@ -307,7 +307,8 @@ int asrk_kv_read(const asrk_kv_cache* c, int layer, int layers, const int32_t* f
 /* Attention over one layer of the cache: row i of sequence s, for i < lens - starts, sees tokens 0 .. starts[s] + i;
  * the other rows become zero.  q bf16 [num_seqs][n][q_heads][head_dim] (strides in values, multiples of 8), q_heads a
  * multiple of kv_heads, scale > 0, out bf16 [num_seqs][n][q_heads][head_dim] dense.  num_beams consecutive sequences are worked on
- * together, and pages that their tables share are read once; it changes no result but for rounding.  num_beams <= 32. */
+ * together, and pages that their tables share are read once; it changes no result but for rounding.  num_beams <= 32,
+ * num_beams n q_heads / kv_heads <= 65535 * 128. */
 size_t asrk_kv_attention_workspace_bytes(const asrk_kv_cache* c, int n, int q_heads, int num_beams);
 int asrk_kv_attention(const asrk_kv_cache* c, int layer, const void* q, int64_t seq_ld, int64_t row_ld, int64_t head_ld, int n,
                       int q_heads, int num_beams, float scale, void* out, void* ws, size_t ws_bytes, void* stream);

@@ -185,3 +185,14 @@ def test_c_abi_refusals():
     assert lib.asrk_reorder_rows(None, p, 2, 5, 16, p, None) == NULL
     assert lib.asrk_reorder_rows(p, p, 2, 5, 0, p, None) == SHAPE and lib.asrk_reorder_rows(p, p, 20000, 5, 16, p, None) == SHAPE
     assert math.isfinite(need)
+
+
+def test_c_abi_refuses_more_columns_than_the_grid_takes():
+    from asr_amd import _lib
+
+    lib = _lib.load()
+    p, c = 1 << 20, _cache_struct(max_pages=100)
+    most = 65535 * 128 // 2  # of two query heads per key/value head
+    assert lib.asrk_kv_attention_workspace_bytes(c, most, 4, 1) > 0 and lib.asrk_kv_attention_workspace_bytes(c, most + 1, 4, 1) == 0
+    assert lib.asrk_kv_attention(c, 0, p, 256, 128, 64, most + 1, 4, 1, 0.125, p, p, 1 << 60, None) == SHAPE
+    assert lib.asrk_kv_attention(c, 0, p, 256, 128, 64, most // 2 + 1, 4, 2, 0.125, p, p, 1 << 60, None) == SHAPE

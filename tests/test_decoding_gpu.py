@@ -623,6 +623,13 @@ def test_attend_keeps_the_queries_nan(n):
     assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], clean[~hit])
 
 
+def test_attend_refuses_more_rows_than_one_call_takes():
+    c, _ = both(1, 64, 1, 64)
+    q = torch.zeros((1, 1, 4, 64), device="cuda", dtype=torch.bfloat16).expand(1, 65535 * 128 // 4 + 1, 4, 64)
+    with pytest.raises(ValueError, match="one call"):
+        c.attend(q)
+
+
 def test_attend_takes_any_strides():
     rng = np.random.default_rng(10)
     c, o = filled(rng, 3, 2, 64, [70, 3, 100], [2, 2, 2], layers=2)

@@ -239,7 +239,7 @@ __device__ __forceinline__ double from_lane(double v) {  // 0 where there is non
     return __longlong_as_double((int64_t)(((uint64_t)high << 32) | low));
 }
 __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __restrict__ keys, const float2* __restrict__ stats,
-                                                           const float* __restrict__ scores, int K, int V, int chunks, int n,
+                                                           const float* __restrict__ scores, int K, int V, int chunks, int n, float chunks_inv, float n_inv,
                                                            int64_t eos, float* __restrict__ out_scores,
                                                            int64_t* __restrict__ out_tokens, int64_t* __restrict__ out_parents,
                                                            float* __restrict__ cand_scores, int64_t* __restrict__ cand_tokens,
@@ -299,7 +299,6 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
 #pragma unroll
     for (int q = 0; q < JOIN_HELD; ++q) ahead_keys[q * JOIN_T + threadIdx.x] = held[q];
     __syncthreads();
-    const float n_inv = 1.f / (float)n, chunks_inv = 1.f / (float)chunks;
     // entry j of list l, whose key is `key`; false: none
     auto entry = [&](int l, int j, uint64_t key, Pick& p) -> bool {
         const int k = over(l, chunks_inv);
@@ -435,7 +434,7 @@ extern "C" int asrk_beam_select(const void* logits, int dtype, int64_t ld, const
         hipLaunchKernelGGL((beam_chunk_kernel<bf16_t, 32>), grid, dim3(256), lds, st, (const bf16_t*)logits, ld, V, 2 * K, keys, stats);
     else
         hipLaunchKernelGGL((beam_chunk_kernel<bf16_t, 64>), grid, dim3(256), lds, st, (const bf16_t*)logits, ld, V, 2 * K, keys, stats);
-    hipLaunchKernelGGL(beam_join_kernel, dim3(B), dim3(JOIN_T), 0, st, keys, stats, scores, K, V, chunks, 2 * K, eos, out_scores,
+    hipLaunchKernelGGL(beam_join_kernel, dim3(B), dim3(JOIN_T), 0, st, keys, stats, scores, K, V, chunks, 2 * K, 1.f / chunks, 0.5f / K, eos, out_scores,
                        out_tokens, out_parents, cand_scores, cand_tokens, cand_parents);
     return hipGetLastError() == hipSuccess ? ASRK_OK : ASRK_ERR_HIP;
 }

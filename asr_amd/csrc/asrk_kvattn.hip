@@ -14,8 +14,8 @@
 // Keys become bf16 with their scale applied (exact); values become f16 in a unit that follows the pages' scales (exact, for
 // pages up to 2^90 apart).  Weights are rounded to f16, 2^-11 relative, 8 times finer than bf16 would be and well under the
 // 2^-8 of the bf16 result.  Everything else is fp32.
-// Measured: 1.2 GB of cache (48 sequences, 8 heads of 128) 204 us = 5.9 TB/s; 64 x 5 beams over 1641 tokens that share their
-// prompts (64 MB) 20 us; one utterance 12 us, latency.
+// Measured: 1.2 GB of cache (48 sequences, 8 heads of 128) 203 us = 5.9 TB/s; 64 x 5 beams over 1641 tokens that share their
+// prompts (64 MB) 19 us; one utterance 11 us, latency, of which fetching the code for the first time is a good part.
 #include "asrk_kvcache.h"
 
 namespace {
@@ -483,11 +483,11 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
 // it is vector instructions, and a fifth of those are conversions, so every page is converted once for the four waves: each
 // converts a quarter, into LDS, in the order in which the products' first operands are read (a lane's 16 bytes after
 // another's: no bank conflict).  Two buffers, one barrier per page; the next page's bytes are on their way meanwhile.
-// 16 prompts of up to 1541 tokens, 15 query heads on 5 of 64: 93 us (440 TFLOP/s; every wave converting for itself 105); of 4096
-// tokens 720 TFLOP/s, with heads of 128 830.  Of a wave's vector issue slots 60 % are used: the rest is the prologue of short
+// 16 prompts of up to 1541 tokens, 15 query heads on 5 of 64: 89 us (460 TFLOP/s; every wave converting for itself 105); of 4096
+// tokens 740 TFLOP/s, with heads of 128 835.  Of a wave's vector issue slots 60 % are used: the rest is the prologue of short
 // rows and waves of a workgroup waiting for each other.
 constexpr int PROMPT_W = 4, PROMPT_CT = 2;
-// (D 64: 4 waves per SIMD, a few spilled registers included: 16 prompts of 4096 tokens 715 us; 3 waves 738 when it was 684.)
+// (D 64: 4 waves per SIMD, a few spilled registers included, are 7 % faster than 3.)
 constexpr int prompt_occupancy(int D) { return D == 64 ? 4 : 2; }
 template <int D>
 __global__ __launch_bounds__(64 * PROMPT_W) __attribute__((amdgpu_waves_per_eu(prompt_occupancy(D), prompt_occupancy(D))))

@@ -328,11 +328,12 @@ class PagedKVCache:
         if layers * self.num_seqs > 65535:
             raise ValueError("read one layer at a time: layers * num_seqs passes 65535")
         shape = (self.num_seqs, count, self.kv_heads, self.head_dim)
-        out = [torch.empty(shape if layer is not None else (layers, *shape), dtype=torch.bfloat16, device=self.device) for _ in range(2)]
+        k = torch.empty(shape if layer is not None else (layers, *shape), dtype=torch.bfloat16, device=self.device)
+        v = torch.empty_like(k)
         layer = 0 if layer is None else self._layer(layer)
         if count:
-            _call("asrk_kv_read", self.device, self._ref, layer, layers, _address(each), first, count, out[0].data_ptr(), out[1].data_ptr())
-        return out[0], out[1]
+            _call("asrk_kv_read", self.device, self._ref, layer, layers, _address(each), first, count, k.data_ptr(), v.data_ptr())
+        return k, v
 
     def attend(self, q: torch.Tensor, layer: int = 0, *, scale: Optional[float] = None, num_beams: int = 1) -> torch.Tensor:
         """Attention of the new tokens over one layer of the cache: bfloat16 [num_seqs, n, q_heads, head_dim] for ``q`` of that

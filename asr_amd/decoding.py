@@ -250,7 +250,7 @@ class PagedKVCache:
         if self._seq_stride != 1:
             raise ValueError("compact the cache itself, not a view of some of its sequences")
         _call("asrk_kv_compact", self.device, self._ref)
-        return self.status[1]
+        return self.status[1].clone()  # the word itself is the next compaction's
 
     def check(self) -> None:
         """Raises if any call since the last ``check`` could not be carried out (one host synchronisation)."""

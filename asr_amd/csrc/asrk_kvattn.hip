@@ -11,9 +11,9 @@
 //   O^T = V^T P^T (16x16x32 f16)   the lane's 16 weights are the second operand as they are, and 16 consecutive tokens of
 //                                  one d are 16 bytes of the value page
 // Columns are the rows of q that share a key/value head: beams x new tokens x query heads per key/value head.
-// Keys become bf16 with their scale applied (exact); values become f16 in a unit that follows the pages' scales (exact, for
-// pages up to 2^90 apart).  Weights are rounded to f16, 2^-11 relative, 8 times finer than bf16 would be and well under the
-// 2^-8 of the bf16 result.  Everything else is fp32.
+// Keys become bf16 with their scale applied (exact); values become f16 in a unit that follows the pages' scales (exact, see
+// Unit).  Weights are rounded to f16, 2^-11 relative, 8 times finer than bf16 would be and well under the 2^-8 of the bf16
+// result.  Everything else is fp32.
 // Measured: 1.2 GB of cache (48 sequences, 8 heads of 128) 203 us = 5.9 TB/s; 64 x 5 beams over 1641 tokens that share their
 // prompts (64 MB) 19 us; one utterance 11 us, latency, of which fetching the code for the first time is a good part.
 #include "asrk_kvcache.h"
@@ -137,7 +137,7 @@ struct Queries {
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             const int s = limit[t] - p * ASRK_KV_PAGE;
-            const bool takes = (with >> beam[t]) & 1;
+            const bool takes = ((uint32_t)with >> beam[t]) & 1;  // 32 beams at most: one register
             seen[t] = limit[t] == NO_COLUMN || (takes && s > ASRK_KV_PAGE) ? ASRK_KV_PAGE : (takes && s > 0 ? s : 0);
             all = seen[t] < all ? seen[t] : all;
             some = seen[t] > some && limit[t] != NO_COLUMN ? seen[t] : some;
@@ -156,8 +156,8 @@ struct Pages {
     const int* table;  // of beam `lane`
     int beams, max_pages, num_pages, lane, at_p, step, item_p, mine, coming;
     uint64_t left;
-    __device__ __forceinline__ Pages(const asrk_kv_cache& c, int beams_, int set, int first, int step_)
-        : beams(beams_), max_pages(c.max_pages), num_pages(c.num_pages), lane(threadIdx.x & 63), at_p(first), step(step_), item_p(0),
+    __device__ __forceinline__ Pages(const asrk_kv_cache& c, int beams_, int set, int first, int step_, int lane_)
+        : beams(beams_), max_pages(c.max_pages), num_pages(c.num_pages), lane(lane_), at_p(first), step(step_), item_p(0),
           mine(-1), left(0) {
         table = c.table + ((int64_t)set * beams + lane) * c.seq_stride * max_pages;
         coming = number(first);
@@ -196,16 +196,19 @@ __device__ __forceinline__ u32x4 keep_before(int last, int g) {
     return mask;
 }
 // Values are multiplied, and o is held, in units of 2^now.  An e4m3 value times 2^-15 .. 2^7 is exact in f16, so the unit
-// stays while a page's exponent lies in that window, and else follows it up or down -- down at most 2^75 below the largest
-// exponent so far, where o cannot leave fp32's range yet.  (A unit that only rises would round the values of a beam, or of a
-// page, by those of another that happens to come before.)
+// stays while a page's exponent lies in that window, and else follows it up or down.  (A unit that only rises would round the
+// values of a beam, or of a page, by those of another that happens to come before.)  That does while all exponents so far lie
+// within 2^64: o, at most 2^(64 + 7) times what a page adds to it (2^24 per token at most), cannot leave fp32's range then.
+// Exponents further apart -- of beams that are worked on together, or of pages whose weights make up for it or not -- leave no
+// unit in which f16 holds both: walk_apart() takes over.
 struct Unit {
-    int now = ASRK_KV_EXP_MIN, top = ASRK_KV_EXP_MIN;
-    __device__ __forceinline__ int follow(int ev) {
-        top = ev > top ? ev : top;
+    int now = ASRK_KV_EXP_MIN, low = ASRK_KV_EXP_MAX, high = ASRK_KV_EXP_MIN;
+    __device__ __forceinline__ bool follow(int ev) {  // false: too far apart
+        low = ev < low ? ev : low;
+        high = ev > high ? ev : high;
         const int d = ev - now;
-        if (d > 7 || d < -15) now = ev > top - 75 ? ev : top - 75;
-        return now;
+        if (d > 7 || d < -15) now = ev;
+        return high - low <= 64;
     }
 };
 
@@ -299,6 +302,86 @@ __device__ __forceinline__ void mark_nans(Load&& raw_value, const int* seen, int
     }
 }
 
+// The pages from `item` on, where exponents lie further apart than one unit can hold: each is multiplied in the unit of its own
+// exponent, from zero, and added to o in fp32, in units of 2^APART: all that a page can add lies in fp32's range (2^(119 + 9 +
+// 15 - 44) per token at most).  Rare, so it must not cost the other loop registers: each wave reads and converts for itself, and
+// takes one tile of anything at a time.
+constexpr int APART = 44;
+template <int D, int CT>
+__device__ __forceinline__ void walk_apart(Item item, Pages& work, int pages, const Queries<D, CT>& qs, const Columns& cs, const char* layer,
+                                           const int* exps, int lane, float* m, f32x4* l, f32x4 (*o)[D / 16]) {
+    constexpr int KS = D / 64, DT = D / 16;
+    const int col = lane & 15, g = lane >> 4;
+    for (; item.page >= 0; item = work.next(pages)) {
+        int seen[CT];
+        bool whole;
+        if (!qs.see(item.p, item.with, seen, whole)) continue;
+        const int64_t at = (int64_t)item.page * cs.H + cs.h;
+        const __amdgpu_buffer_rsrc_t rows = page_rows(layer, at, D);
+        const int e = __builtin_amdgcn_readfirstlane(exps[at]);
+        const float ks = pow2((int8_t)e), up = pow2((int8_t)(e >> 8) - APART);
+        const bool odd = (e >> 16) & 1;
+        int last = 0;  // token seen by any column
+#pragma unroll
+        for (int x = 0; x < CT; ++x) last = seen[x] > last && qs.limit[x] != NO_COLUMN ? seen[x] : last;
+        const u32x4 mask = keep_before(wave_imax(last), g);
+        auto value = [&](int d) __attribute__((always_inline)) {
+            return __builtin_amdgcn_raw_buffer_load_b128(rows, (col + 16 * d) * ASRK_KV_PAGE + 16 * g, ASRK_KV_PAGE * D, 0);
+        };
+#pragma unroll
+        for (int x = 0; x < CT; ++x) {  // one tile of columns, of keys, of values at a time
+            f32x4 sc[1][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                __builtin_amdgcn_sched_barrier(0);
+                sc[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const u32x4 raw = __builtin_amdgcn_raw_buffer_load_b128(rows, (16 * (col >> 2) + 4 * t + (col & 3)) * D + 64 * s + 16 * g, 0, 0);
+                    sc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8(raw[0], raw[1], ks), qs.q[x][2 * s], sc[0][t], 0, 0, 0);
+                    sc[0][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k8(raw[2], raw[3], ks), qs.q[x][2 * s + 1], sc[0][t], 0, 0, 0);
+                }
+            }
+            f16x8 pf[1][2];
+            weigh<1, DT>(sc, seen + x, whole, g, cs.a.c, APART, APART, m + x, l + x, o + x, pf);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                __builtin_amdgcn_sched_barrier(0);
+                u32x4 raw = value(d) & mask;
+                if (odd)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) raw[w] &= ~nan_bytes(raw[w]);
+                f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < 2; ++u) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8(raw[2 * u], raw[2 * u + 1], 1.f), pf[0][u], sum, 0, 0, 0);
+                o[x][d] += sum * up;
+            }
+            add_weights<1>(pf, l + x);
+            if (odd) mark_nans<1, DT>(value, seen + x, g, o + x);
+        }
+    }
+}
+
+// The same from the first page on, with nothing of what the other loop holds: if it went on from there, that loop would be cut
+// for both (two spilled registers more in kv_prompt_kernel<64>, 10 % of the time of 16 prompts).  Its presence still costs 1 to 4 %.
+template <int D, int CT>
+__device__ __forceinline__ void walk_apart_anew(const asrk_kv_cache& c, const Columns& cs, int first_col, int first_page, int step, int pages,
+                                                const char* layer, const int* exps, float* m, f32x4* l, f32x4 (*o)[D / 16]) {
+    int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    asm volatile("" : "+v"(lane));  // what follows from it is computed and loaded again
+    Pages work(c, cs.a.beams, cs.set, first_page, step, lane);
+    Queries<D, CT> qs;
+    qs.load(c, cs, first_col, lane & 15, lane >> 4);
+#pragma unroll
+    for (int x = 0; x < CT; ++x) {
+        m[x] = NEG_INF;
+        l[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[x][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    walk_apart<D, CT>(work.next(pages), work, pages, qs, cs, layer, exps, lane, m, l, o);
+}
+
 // f over groups of W lanes, in all of them.
 template <int W, class F>
 __device__ __forceinline__ float among(float v, F&& f) {
@@ -328,7 +411,7 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     const Columns cs(c, a, set);
     const int first_col = blockIdx.z * 16 * CT;
     // The pages of a wave: by its number alone, so that their numbers are on the way before the lengths are known.
-    Pages work(c, a.beams, set, part * W + wave, a.splits * W);
+    Pages work(c, a.beams, set, part * W + wave, a.splits * W, lane);
     Queries<D, CT> qs;
     qs.load(c, cs, first_col, col, g);
     const int pages = (wave_imax(qs.most) + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
@@ -361,78 +444,87 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
     Item item = work.next(pages);
     int64_t at = (int64_t)(item.page < 0 ? 0 : item.page) * cs.H + cs.h;
     __amdgpu_buffer_rsrc_t rows = page_rows(layer, at, D);
-    int e_next = 0;
+    bool apart = false;
     if (item.page >= 0) {
-        e_next = exps[at];
+        int e_next = exps[at];
         load_keys(rows);
 #pragma unroll
         for (int d = 0; d < DT; ++d) vr[d] = load_value(rows, d);
-    }
-    while (item.page >= 0) {
-        const Item following = work.next(pages);
-        at = (int64_t)(following.page < 0 ? 0 : following.page) * cs.H + cs.h;
-        const __amdgpu_buffer_rsrc_t rows_next = page_rows(layer, at, D);
-        const int e = __builtin_amdgcn_readfirstlane(e_next);
-        if (following.page >= 0) e_next = exps[at];
-        int seen[CT];
-        bool whole;
-        qs.see(item.p, item.with, seen, whole);
+        for (;;) {
+            const int e = __builtin_amdgcn_readfirstlane(e_next), ev = (int8_t)(e >> 8);
+            if (__builtin_expect(!unit.follow(ev), 0)) {
+                apart = true;
+                break;
+            }
+            const int up = unit.now;
+            const Item following = work.next(pages);
+            at = (int64_t)(following.page < 0 ? 0 : following.page) * cs.H + cs.h;
+            const __amdgpu_buffer_rsrc_t rows_next = page_rows(layer, at, D);
+            if (following.page >= 0) e_next = exps[at];
+            int seen[CT];
+            bool whole;
+            qs.see(item.p, item.with, seen, whole);
 
-        const float ks = pow2((int8_t)e);
-        const int ev = (int8_t)(e >> 8), up = unit.follow(ev);
-        f32x4 sc[CT][4];
+            const float ks = pow2((int8_t)e);
+            f32x4 sc[CT][4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < 4; ++t) {
 #pragma unroll
-            for (int x = 0; x < CT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int x = 0; x < CT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const bf16x8 k0 = k8(kr[t][s][0], kr[t][s][1], ks), k1 = k8(kr[t][s][2], kr[t][s][3], ks);
+                for (int s = 0; s < KS; ++s) {
+                    const bf16x8 k0 = k8(kr[t][s][0], kr[t][s][1], ks), k1 = k8(kr[t][s][2], kr[t][s][3], ks);
 #pragma unroll
-                for (int x = 0; x < CT; ++x) {
-                    sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qs.q[x][2 * s], sc[x][t], 0, 0, 0);
-                    sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qs.q[x][2 * s + 1], sc[x][t], 0, 0, 0);
+                    for (int x = 0; x < CT; ++x) {
+                        sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qs.q[x][2 * s], sc[x][t], 0, 0, 0);
+                        sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qs.q[x][2 * s + 1], sc[x][t], 0, 0, 0);
+                    }
                 }
             }
-        }
-        if (following.page >= 0) load_keys(rows_next);
-        f16x8 pf[CT][2];
-        weigh<CT, DT>(sc, seen, whole, g, a.c, up, held_unit, m, l, o, pf);
-        held_unit = up;
-        const float vs = pow2(ev - up);
-        if (!whole) {
-            KEEP_BRANCH();
-            int last = 0;  // token seen by any column
+            if (following.page >= 0) load_keys(rows_next);
+            f16x8 pf[CT][2];
+            weigh<CT, DT>(sc, seen, whole, g, a.c, up, held_unit, m, l, o, pf);
+            held_unit = up;
+            const float vs = pow2(ev - up);
+            if (!whole) {
+                KEEP_BRANCH();
+                int last = 0;  // token seen by any column
 #pragma unroll
-            for (int x = 0; x < CT; ++x) last = seen[x] > last && qs.limit[x] != NO_COLUMN ? seen[x] : last;
-            const u32x4 mask = keep_before(wave_imax(last), g);
+                for (int x = 0; x < CT; ++x) last = seen[x] > last && qs.limit[x] != NO_COLUMN ? seen[x] : last;
+                const u32x4 mask = keep_before(wave_imax(last), g);
 #pragma unroll
-            for (int d = 0; d < DT; ++d) vr[d] &= mask;
-        }
-        const bool odd = __builtin_expect((e >> 16) & 1, 0);
-        if (odd) {
-            KEEP_BRANCH();
+                for (int d = 0; d < DT; ++d) vr[d] &= mask;
+            }
+            const bool odd = __builtin_expect((e >> 16) & 1, 0);
+            if (odd) {
+                KEEP_BRANCH();
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) vr[d][w] &= ~nan_bytes(vr[d][w]);
+            }
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) vr[d][w] &= ~nan_bytes(vr[d][w]);
-        }
+                for (int u = 0; u < 2; ++u) {
+                    const f16x8 v = v8(vr[d][2 * u], vr[d][2 * u + 1], vs);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+                    for (int x = 0; x < CT; ++x) o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[x][u], o[x][d], 0, 0, 0);
+                }
+            add_weights<CT>(pf, l);
+            if (odd) mark_nans<CT, DT>([&](int d) { return load_value(rows, d); }, seen, g, o);
+            if (following.page >= 0) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const f16x8 v = v8(vr[d][2 * u], vr[d][2 * u + 1], vs);
-#pragma unroll
-                for (int x = 0; x < CT; ++x) o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[x][u], o[x][d], 0, 0, 0);
+                for (int d = 0; d < DT; ++d) vr[d] = load_value(rows_next, d);
             }
-        add_weights<CT>(pf, l);
-        if (odd) mark_nans<CT, DT>([&](int d) { return load_value(rows, d); }, seen, g, o);
-        if (following.page >= 0) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d) vr[d] = load_value(rows_next, d);
+            if (following.page < 0) break;
+            item = following;
+            rows = rows_next;
         }
-        item = following;
-        rows = rows_next;
+    }
+    if (__builtin_expect(apart, 0)) {
+        held_unit = APART;
+        walk_apart_anew<D, CT>(c, cs, first_col, part * W + wave, a.splits * W, pages, layer, exps, m, l, o);
     }
 
     // ---- join the waves, one column tile at a time
@@ -502,7 +594,7 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
     const int part = part_of(a), set = blockIdx.y, chunk = gridDim.z - 1 - blockIdx.z;
     const Columns cs(c, a, set);
     const int first_col = (chunk * W + wave) * 16 * CT;
-    Pages work(c, a.beams, set, part, a.splits);
+    Pages work(c, a.beams, set, part, a.splits, lane);
     // Tokens of each beam (lane), and how many of them any column of the workgroup sees: of one sequence those up to its last
     // row's own, of several at most all.
     const int64_t seq = (int64_t)set * a.beams;
@@ -564,87 +656,96 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
     Item item = work.next(pages);
     int64_t at = (int64_t)(item.page < 0 ? 0 : item.page) * cs.H + cs.h;
     __amdgpu_buffer_rsrc_t rows = page_rows(layer, at, D);
-    int e_next = 0;
-    if (item.page >= 0) {
-        e_next = exps[at];
-        load_page(rows);
-    }
     char* buf = tiles;
-    while (item.page >= 0) {
-        const Item following = work.next(pages);
-        at = (int64_t)(following.page < 0 ? 0 : following.page) * cs.H + cs.h;
-        const __amdgpu_buffer_rsrc_t rows_next = page_rows(layer, at, D);
-        const int e = __builtin_amdgcn_readfirstlane(e_next);
-        if (following.page >= 0) e_next = exps[at];
-        const int ev = (int8_t)(e >> 8), up = unit.follow(ev);
-        const bool odd = __builtin_expect((e >> 16) & 1, 0);
-        {
-            const float ks = pow2((int8_t)e), vs = pow2(ev - up);
-            const int held = (a.beams == 1 ? __builtin_amdgcn_readfirstlane(held_by)
-                                           : wave_imax((item.with >> lane) & 1 ? held_by : 0)) - item.p * ASRK_KV_PAGE;
-            if (held < ASRK_KV_PAGE) {  // the sequence ends within the page
-                KEEP_BRANCH();
-                const u32x4 mask = keep_before(held, g);
-#pragma unroll
-                for (int d = 0; d < OWN; ++d) vr[d] &= mask;
+    bool apart = false;  // alike in all waves
+    if (item.page >= 0) {
+        int e_next = exps[at];
+        load_page(rows);
+        for (;;) {
+            const int e = __builtin_amdgcn_readfirstlane(e_next), ev = (int8_t)(e >> 8);
+            if (__builtin_expect(!unit.follow(ev), 0)) {
+                apart = true;
+                break;
             }
-            if (odd) {
-                KEEP_BRANCH();
+            const int up = unit.now;
+            const Item following = work.next(pages);
+            at = (int64_t)(following.page < 0 ? 0 : following.page) * cs.H + cs.h;
+            const __amdgpu_buffer_rsrc_t rows_next = page_rows(layer, at, D);
+            if (following.page >= 0) e_next = exps[at];
+            const bool odd = __builtin_expect((e >> 16) & 1, 0);
+            {
+                const float ks = pow2((int8_t)e), vs = pow2(ev - up);
+                const int held = (a.beams == 1 ? __builtin_amdgcn_readfirstlane(held_by)
+                                               : wave_imax((item.with >> lane) & 1 ? held_by : 0)) - item.p * ASRK_KV_PAGE;
+                if (held < ASRK_KV_PAGE) {  // the sequence ends within the page
+                    KEEP_BRANCH();
+                    const u32x4 mask = keep_before(held, g);
 #pragma unroll
-                for (int d = 0; d < OWN; ++d)
+                    for (int d = 0; d < OWN; ++d) vr[d] &= mask;
+                }
+                if (odd) {
+                    KEEP_BRANCH();
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) vr[d][w] &= ~nan_bytes(vr[d][w]);
-            }
-            // fragment (tile, step): 64 lanes of 16 bytes
+                    for (int d = 0; d < OWN; ++d)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                bf16x8* to = reinterpret_cast<bf16x8*>(buf) + (wave * 2 * KS + 2 * s) * 64 + lane;
-                to[0] = k8(kr[s][0], kr[s][1], ks);
-                to[64] = k8(kr[s][2], kr[s][3], ks);
-            }
+                        for (int w = 0; w < 4; ++w) vr[d][w] &= ~nan_bytes(vr[d][w]);
+                }
+                // fragment (tile, step): 64 lanes of 16 bytes
 #pragma unroll
-            for (int d = 0; d < OWN; ++d) {
-                f16x8* to = reinterpret_cast<f16x8*>(buf + K_BYTES) + (wave * OWN + d) * 128 + lane;
-                to[0] = v8(vr[d][0], vr[d][1], vs);
-                to[64] = v8(vr[d][2], vr[d][3], vs);
-            }
-        }
-        __syncthreads();  // the other buffer was last read before the barrier in front of this one
-        if (following.page >= 0) load_page(rows_next);
-        int seen[CT];
-        bool whole;
-        if (qs.see(item.p, item.with, seen, whole)) {
-            const bf16x8* kt = reinterpret_cast<const bf16x8*>(buf) + lane;
-            const f16x8* vt = reinterpret_cast<const f16x8*>(buf + K_BYTES) + lane;
-            f32x4 sc[CT][4];
+                for (int s = 0; s < KS; ++s) {
+                    bf16x8* to = reinterpret_cast<bf16x8*>(buf) + (wave * 2 * KS + 2 * s) * 64 + lane;
+                    to[0] = k8(kr[s][0], kr[s][1], ks);
+                    to[64] = k8(kr[s][2], kr[s][3], ks);
+                }
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                for (int x = 0; x < CT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = 0; s < 2 * KS; ++s) {
-                    const bf16x8 k = kt[(t * 2 * KS + s) * 64];
-#pragma unroll
-                    for (int x = 0; x < CT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qs.q[x][s], sc[x][t], 0, 0, 0);
+                for (int d = 0; d < OWN; ++d) {
+                    f16x8* to = reinterpret_cast<f16x8*>(buf + K_BYTES) + (wave * OWN + d) * 128 + lane;
+                    to[0] = v8(vr[d][0], vr[d][1], vs);
+                    to[64] = v8(vr[d][2], vr[d][3], vs);
                 }
             }
-            f16x8 pf[CT][2];
-            weigh<CT, DT>(sc, seen, whole, g, a.c, up, held_unit, m, l, o, pf);
-            held_unit = up;
+            __syncthreads();  // the other buffer was last read before the barrier in front of this one
+            if (following.page >= 0) load_page(rows_next);
+            int seen[CT];
+            bool whole;
+            if (qs.see(item.p, item.with, seen, whole)) {
+                const bf16x8* kt = reinterpret_cast<const bf16x8*>(buf) + lane;
+                const f16x8* vt = reinterpret_cast<const f16x8*>(buf + K_BYTES) + lane;
+                f32x4 sc[CT][4];
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+                for (int t = 0; t < 4; ++t) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const f16x8 v = vt[(d * 2 + u) * 64];
+                    for (int x = 0; x < CT; ++x) sc[x][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int x = 0; x < CT; ++x) o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[x][u], o[x][d], 0, 0, 0);
+                    for (int s = 0; s < 2 * KS; ++s) {
+                        const bf16x8 k = kt[(t * 2 * KS + s) * 64];
+#pragma unroll
+                        for (int x = 0; x < CT; ++x) sc[x][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qs.q[x][s], sc[x][t], 0, 0, 0);
+                    }
                 }
-            add_weights<CT>(pf, l);
-            if (odd) mark_nans<CT, DT>([&](int d) { return load_value(rows, d); }, seen, g, o);
+                f16x8 pf[CT][2];
+                weigh<CT, DT>(sc, seen, whole, g, a.c, up, held_unit, m, l, o, pf);
+                held_unit = up;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const f16x8 v = vt[(d * 2 + u) * 64];
+#pragma unroll
+                        for (int x = 0; x < CT; ++x) o[x][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[x][u], o[x][d], 0, 0, 0);
+                    }
+                add_weights<CT>(pf, l);
+                if (odd) mark_nans<CT, DT>([&](int d) { return load_value(rows, d); }, seen, g, o);
+            }
+            buf = buf == tiles ? tiles + BUF : tiles;
+            if (following.page < 0) break;
+            item = following;
+            rows = rows_next;
         }
-        buf = buf == tiles ? tiles + BUF : tiles;
-        item = following;
-        rows = rows_next;
+    }
+    if (__builtin_expect(apart, 0)) {
+        held_unit = APART;
+        walk_apart_anew<D, CT>(c, cs, first_col, part, a.splits, pages, layer, exps, m, l, o);
     }
 #pragma unroll
     for (int x = 0; x < CT; ++x) {

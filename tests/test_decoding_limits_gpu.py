@@ -34,3 +34,101 @@ def test_compact_results_stay():
     assert len({want for _, want in used}) == 3
     assert [int(got) for got, _ in used] == [want for _, want in used]
     assert all(got.dtype == torch.int32 and got.dim() == 0 for got, _ in used)
+
+
+# ---- attention
+
+
+def put(c, o, k, v):
+    c.write(k, v)
+    o.write(k.double().cpu().numpy(), v.double().cpu().numpy())
+
+
+def normal(rng, *shape):
+    return torch.from_numpy(rng.standard_normal(shape)).float().cuda()
+
+
+@pytest.mark.parametrize("gap", [110, 150])
+@pytest.mark.parametrize("large", [0, 1])
+@pytest.mark.parametrize("n,group,dim", [(1, 3, 64), (1, 20, 64), (1, 4, 128), (50, 2, 64), (70, 3, 128)])
+def test_attend_beams_whose_scales_lie_very_far_apart(gap, large, n, group, dim):
+    """Beams whose values are 2**gap apart, worked on together and alone: neither costs the other anything."""
+    rng = np.random.default_rng(gap + large)
+    c, o = both(2, 1100, 1, dim)
+    size = torch.full((2, 1, 1, 1), 2.0 ** (40 - gap), device="cuda")
+    size[large] = 2.0 ** 40
+    for rows in (1000, n):  # two pages for each of eight waves
+        c.extend(rows)
+        o.extend(rows)
+        put(c, o, normal(rng, 2, rows, 1, dim), normal(rng, 2, rows, 1, dim) * size)
+    q = torch.from_numpy(rng.standard_normal((2, n, group, dim))).cuda().bfloat16()
+    same_attention(c, o, q, beams=2, name="together")
+    same_attention(c, o, q, name="alone")
+
+
+@pytest.mark.parametrize("n,group", [(1, 3), (1, 12), (30, 4)])
+def test_attend_shared_pages_before_tails_of_every_scale(n, group):
+    """Beams that share a prompt of ordinary values and go on with tiny, ordinary and enormous ones."""
+    rng = np.random.default_rng(n)
+    S = 3
+    c, o = both(S, 1500, 1, 64)
+    lead = c.leaders(S)
+    lead.extend(700)
+    o.extend([700], S)
+    k, v = normal(rng, 1, 700, 1, 64), normal(rng, 1, 700, 1, 64)
+    lead.write(k, v)
+    o.write(k.double().cpu().numpy(), v.double().cpu().numpy(), every=S)
+    c.reorder(torch.zeros((1, S), dtype=torch.int64, device="cuda"))
+    o.reorder([[0] * S])
+    size = torch.tensor([2.0 ** 115, 1.0, 2.0 ** -50], device="cuda").view(S, 1, 1, 1)
+    for rows in (650, n):
+        c.extend(rows)
+        o.extend(rows)
+        put(c, o, normal(rng, S, rows, 1, 64), normal(rng, S, rows, 1, 64) * size)
+    q = torch.from_numpy(rng.standard_normal((S, n, group, 64))).cuda().bfloat16()
+    same_attention(c, o, q, beams=S)
+    same_attention(c, o, q)
+
+
+@pytest.mark.parametrize("scales", [(110, 0), (0, 110), (119, -60, 30), (-60, 119, -60, 100), (30, 119, -40, 0, 90, -60)])
+@pytest.mark.parametrize("n,max_len", [(1, 1500), (1, 4000), (1, 64 * 60), (140, 1500), (140, 4000)])
+def test_attend_enormous_values_that_weigh_nothing(scales, n, max_len):
+    """Pages of enormous values whose scores are far below the others': the small values are the result, to their own size."""
+    rng = np.random.default_rng(len(scales) + n)
+    c, o = both(1, max_len, 1, 64)
+    dark = torch.zeros((64,), device="cuda")
+    dark[0] = 1.0
+    for step in range(12):
+        e = scales[step % len(scales)]
+        c.extend(100)
+        o.extend(100)
+        k, v = normal(rng, 1, 100, 1, 64), normal(rng, 1, 100, 1, 64) * 2.0 ** e
+        k[..., 0] = -300.0 * (e > min(scales))  # times q's 8 / 8
+        put(c, o, k, v)
+    c.extend(n)
+    o.extend(n)
+    put(c, o, normal(rng, 1, n, 1, 64) * (1 - dark), normal(rng, 1, n, 1, 64) * 2.0 ** min(scales))
+    q = torch.from_numpy(rng.standard_normal((1, n, 2, 64))).cuda().bfloat16()
+    q[..., 0] = 8
+    same_attention(c, o, q)
+
+
+@pytest.mark.parametrize("n,group,dim", [(1, 3, 64), (3, 9, 64), (40, 4, 64), (1, 2, 128), (2, 16, 128), (40, 4, 128)])
+def test_attend_far_apart_with_nan_ended_sequences_and_short_tails(n, group, dim):
+    """Scales that no unit holds, of sequences of which one has ended, with numbers that are not finite in places that some rows
+    see and some do not, and memory behind the last tokens that holds NaN bytes."""
+    rng = np.random.default_rng(n + dim)
+    S = 4
+    c, o = both(S, 900, 2, dim)
+    size = torch.tensor([2.0 ** 118, 1.0, 2.0 ** -55, 2.0 ** 30], device="cuda").view(S, 1, 1, 1)
+    for rows in ([700, 650, 64, 130], [n, max(1, n - 1), 0, n]):
+        c.extend(torch.tensor(rows, device="cuda"))
+        o.extend(rows)
+        k, v = normal(rng, S, max(rows), 2, dim), normal(rng, S, max(rows), 2, dim) * size
+        if max(rows) == n:
+            v[0, n - 1, 1, 5], v[1, 0, 0, dim - 1], k[3, n // 2, 0, 3] = math.inf, math.nan, math.nan
+        put(c, o, k, v)
+    q = torch.from_numpy(rng.standard_normal((S, n, 2 * group, dim))).cuda().bfloat16()
+    same_attention(c, o, q, beams=4)
+    same_attention(c, o, q, beams=2)
+    assert int((c.attend(q, num_beams=4)[2] != 0).sum()) == 0

@@ -595,18 +595,21 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
     const Columns cs(c, a, set);
     const int first_col = (chunk * W + wave) * 16 * CT;
     Pages work(c, a.beams, set, part, a.splits, lane);
-    // Tokens of each beam (lane), and how many of them any column of the workgroup sees: of one sequence those up to its last
-    // row's own, of several at most all.
+    // How many tokens any column of the workgroup sees, of one sequence (up to its last row's own) or of each of several (lane).
+    // What lies behind them in a page may not have been written yet, and may be anything.
     const int64_t seq = (int64_t)set * a.beams;
-    const int held_by = lane < a.beams ? c.lens[(seq + lane) * c.seq_stride] : 0;
-    int most;
+    int most, seen_of = 0;
     if (a.beams == 1) {
-        const int start = c.starts[seq * c.seq_stride], fresh = __builtin_amdgcn_readfirstlane(held_by) - start;
+        const int start = c.starts[seq * c.seq_stride], fresh = c.lens[seq * c.seq_stride] - start;
         const int x0 = chunk * W * 16 * CT, x1 = x0 + W * 16 * CT < cs.columns ? x0 + W * 16 * CT : cs.columns;
         const int i0 = over(x0, a.group_inv), i1 = over(x1 - 1, a.group_inv) + 1;
         most = i0 >= fresh ? 0 : start + (i1 < fresh ? i1 : fresh);
     } else {
-        most = wave_imax(held_by);
+        if (lane < a.beams) {
+            const int start = c.starts[(seq + lane) * c.seq_stride], fresh = c.lens[(seq + lane) * c.seq_stride] - start;
+            seen_of = fresh <= 0 ? 0 : start + (fresh < a.n ? fresh : a.n);
+        }
+        most = wave_imax(seen_of);
     }
     int pages = (most + ASRK_KV_PAGE - 1) / ASRK_KV_PAGE;
     pages = pages < c.max_pages ? pages : c.max_pages;
@@ -675,11 +678,10 @@ void kv_prompt_kernel(asrk_kv_cache c, AttnArgs a) {
             const bool odd = __builtin_expect((e >> 16) & 1, 0);
             {
                 const float ks = pow2((int8_t)e), vs = pow2(ev - up);
-                const int held = (a.beams == 1 ? __builtin_amdgcn_readfirstlane(held_by)
-                                               : wave_imax((item.with >> lane) & 1 ? held_by : 0)) - item.p * ASRK_KV_PAGE;
-                if (held < ASRK_KV_PAGE) {  // the sequence ends within the page
+                const int last = (a.beams == 1 ? most : wave_imax((item.with >> lane) & 1 ? seen_of : 0)) - item.p * ASRK_KV_PAGE;
+                if (last < ASRK_KV_PAGE) {  // within the page
                     KEEP_BRANCH();
-                    const u32x4 mask = keep_before(held, g);
+                    const u32x4 mask = keep_before(last, g);
 #pragma unroll
                     for (int d = 0; d < OWN; ++d) vr[d] &= mask;
                 }

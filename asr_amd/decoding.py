@@ -290,8 +290,9 @@ class PagedKVCache:
 
     def write(self, k: torch.Tensor, v: torch.Tensor, layer: int = 0) -> None:
         """The new tokens' keys and values of one layer: ``k``, ``v`` [num_seqs, n, kv_heads, head_dim] (float32 or bfloat16, any
-        strides).  Row i of sequence s is its token ``starts[s] + i``; rows behind ``lens[s]`` are not looked at, and new tokens
-        that no row is given for are not written."""
+        strides).  Row i of sequence s is its token ``starts[s] + i``; rows behind ``lens[s]`` are not looked at.  New tokens that
+        no row is given for are not written, and hold nothing defined until they are (also if an earlier call wrote them: a page's
+        scale is that of the rows it was given last)."""
         shape = k.shape
         if len(shape) != 4 or shape != v.shape or shape[0] != self.num_seqs or shape[2] != self.kv_heads or shape[3] != self.head_dim:
             raise ValueError(f"k and v must be [{self.num_seqs}, n, {self.kv_heads}, {self.head_dim}], got {list(shape)} and {list(v.shape)}")
@@ -338,7 +339,8 @@ class PagedKVCache:
     def attend(self, q: torch.Tensor, layer: int = 0, *, scale: Optional[float] = None, num_beams: int = 1) -> torch.Tensor:
         """Attention of the new tokens over one layer of the cache: bfloat16 [num_seqs, n, q_heads, head_dim] for ``q`` of that
         shape (any strides; query head j reads key/value head ``j // (q_heads // kv_heads)``).  Row i of sequence s sees the
-        tokens up to its own, ``starts[s] + i``; rows behind ``lens[s]`` are zero.  ``scale`` (positive) is ``head_dim ** -0.5`` by default.
+        tokens up to its own, ``starts[s] + i``; rows behind ``lens[s]`` are zero.  Tokens that a row sees have to have been written;
+        those behind the last row's own need not be yet.  ``scale`` (positive) is ``head_dim ** -0.5`` by default.
 
         ``num_beams`` consecutive sequences are worked on together, and pages that they share are read once.  It changes
         no result but for rounding: the beams may share any pages, or none."""

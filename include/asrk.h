@@ -295,7 +295,8 @@ int asrk_kv_reorder(const asrk_kv_cache* c, const int64_t* parents, int K, void*
 int asrk_kv_compact(const asrk_kv_cache* c, void* stream);
 
 /* Rows 0 .. min(n, lens - starts) - 1 of k and v ([num_seqs][n][kv_heads][head_dim], ASRK_F32 | ASRK_BF16, strides in
- * values, the last dimension dense, 16-byte aligned rows) become the tokens from starts[s] on of one layer. */
+ * values, the last dimension dense, 16-byte aligned rows) become the tokens from starts[s] on of one layer.  New tokens that no
+ * row is given for hold nothing defined until one is. */
 int asrk_kv_write(const asrk_kv_cache* c, int layer, const void* k, const void* v, int dtype, int64_t seq_ld, int64_t row_ld,
                   int64_t head_ld, int n, void* stream);
 
@@ -304,11 +305,11 @@ int asrk_kv_write(const asrk_kv_cache* c, int layer, const void* k, const void* 
 int asrk_kv_read(const asrk_kv_cache* c, int layer, int layers, const int32_t* first_each, int first_all, int count, void* k_out,
                  void* v_out, void* stream);
 
-/* Attention over one layer of the cache: row i of sequence s, for i < lens - starts, sees tokens 0 .. starts[s] + i;
- * the other rows become zero.  q bf16 [num_seqs][n][q_heads][head_dim] (strides in values, multiples of 8), q_heads a
- * multiple of kv_heads, scale > 0, out bf16 [num_seqs][n][q_heads][head_dim] dense.  num_beams consecutive sequences are worked on
- * together, and pages that their tables share are read once; it changes no result but for rounding.  num_beams <= 32,
- * num_beams n q_heads / kv_heads <= 65535 * 128. */
+/* Attention over one layer of the cache: row i of sequence s, for i < lens - starts, sees tokens 0 .. starts[s] + i, which have
+ * to have been written; the other rows become zero.  q bf16 [num_seqs][n][q_heads][head_dim] (strides in values, multiples of
+ * 8), q_heads a multiple of kv_heads, scale > 0, out bf16 [num_seqs][n][q_heads][head_dim] dense.  num_beams consecutive
+ * sequences are worked on together, and pages that their tables share are read once; it changes no result but for rounding.
+ * num_beams <= 32, num_beams n q_heads / kv_heads <= 65535 * 128. */
 size_t asrk_kv_attention_workspace_bytes(const asrk_kv_cache* c, int n, int q_heads, int num_beams);
 int asrk_kv_attention(const asrk_kv_cache* c, int layer, const void* q, int64_t seq_ld, int64_t row_ld, int64_t head_ld, int n,
                       int q_heads, int num_beams, float scale, void* out, void* ws, size_t ws_bytes, void* stream);

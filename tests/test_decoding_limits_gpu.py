@@ -132,3 +132,22 @@ def test_attend_far_apart_with_nan_ended_sequences_and_short_tails(n, group, dim
     same_attention(c, o, q, beams=4)
     same_attention(c, o, q, beams=2)
     assert int((c.attend(q, num_beams=4)[2] != 0).sum()) == 0
+
+
+@pytest.mark.parametrize("beams,before,rows,n,group", [(1, 0, 100, 100, 2), (1, 37, 90, 90, 2), (2, 5, 70, 70, 3), (1, 64, 1, 1, 130), (1, 10, 20, 20, 1), (2, 10, 3, 3, 2)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_before_the_last_new_tokens_are_written(beams, before, rows, n, group, dim):
+    """Room for 200 tokens, `rows` written: the memory of the others holds NaN bytes, and no row that sees written tokens only
+    is touched by them."""
+    rng = np.random.default_rng(rows)
+    S = 2 * beams
+    c, o = both(S, 320, 1, dim)
+    if before:
+        c.extend(before)
+        o.extend(before)
+        put(c, o, normal(rng, S, before, 1, dim), normal(rng, S, before, 1, dim))
+    c.extend(200)
+    o.extend(200)
+    put(c, o, normal(rng, S, rows, 1, dim), normal(rng, S, rows, 1, dim))
+    q = torch.from_numpy(rng.standard_normal((S, min(n, rows), group, dim))).cuda().bfloat16()
+    same_attention(c, o, q, beams=beams)

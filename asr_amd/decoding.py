@@ -308,7 +308,8 @@ class PagedKVCache:
         (k, lds), (v, v_lds) = self._rows(k), self._rows(v)
         if lds != v_lds:
             k, v = k.contiguous(), v.contiguous()
-            lds = k.stride()[:3]
+            row = self.kv_heads * self.head_dim
+            lds = (n * row, row, self.head_dim)  # not k.stride(): a dimension of 1 may have any
         _call("asrk_kv_write", self.device, self._ref, layer, k.data_ptr(), v.data_ptr(), _DT[k.dtype], *lds, n)
 
     def read(self, first: Union[int, torch.Tensor], count: int, layer: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:

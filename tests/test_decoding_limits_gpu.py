@@ -151,3 +151,26 @@ def test_attend_before_the_last_new_tokens_are_written(beams, before, rows, n, g
     put(c, o, normal(rng, S, rows, 1, dim), normal(rng, S, rows, 1, dim))
     q = torch.from_numpy(rng.standard_normal((S, min(n, rows), group, dim))).cuda().bfloat16()
     same_attention(c, o, q, beams=beams)
+
+
+# ---- tokens
+
+
+def test_write_takes_any_stride_of_a_dimension_of_one():
+    """One sequence, one token or one head may lie at any stride, in one of the two tensors or in both."""
+    g = _gen(1)
+    buf = torch.randn((40000,), generator=g, device="cuda").bfloat16()
+    for shape in ((1, 66, 2, 64), (2, 1, 2, 64), (2, 66, 1, 64), (1, 1, 1, 64)):
+        S, n, H, D = shape
+        dense = [n * H * D, H * D, D, 1]
+        for odd in ((i,) for i in range(3) if shape[i] == 1):
+            strides = [st + 3 if i in odd else st for i, st in enumerate(dense)]
+            k = torch.as_strided(buf, shape, strides, 64)
+            v = torch.randn(shape, generator=g, device="cuda").bfloat16()
+            for first, second in ((k, v), (v, k), (k, k)):
+                c, o = both(S, 100, H, D)
+                c.extend(n)
+                o.extend(n)
+                c.write(first, second)
+                o.write(first.double().cpu().numpy(), second.double().cpu().numpy())
+                same_tokens(c, o, 0, 70)

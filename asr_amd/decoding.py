@@ -138,7 +138,7 @@ def reorder_states(states: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
     if B * K > 65535:
         raise ValueError("reorder_states takes at most 65535 beams in all")
     dev = _gpu("reorder_states", states, parents)
-    states = states.contiguous()
+    states = states.resolve_conj().resolve_neg().contiguous()  # x.conj() is the memory of x
     out = torch.empty_like(states)
     if out.numel():
         _call("asrk_reorder_rows", dev, states.data_ptr(), parents.data_ptr(), B, K, states.numel() // (B * K) * states.element_size(),

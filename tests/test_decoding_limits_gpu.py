@@ -174,3 +174,17 @@ def test_write_takes_any_stride_of_a_dimension_of_one():
                 c.write(first, second)
                 o.write(first.double().cpu().numpy(), second.double().cpu().numpy())
                 same_tokens(c, o, 0, 70)
+
+
+# ---- selection
+
+
+def test_reorder_states_of_conjugated_and_negated_views():
+    from asr_amd.decoding import reorder_states
+
+    x = torch.randn((3, 2, 5), generator=_gen(2), device="cuda", dtype=torch.complex64)
+    par = torch.tensor([[1, 0], [0, 0], [1, 1]], device="cuda")
+    at = (torch.arange(3, device="cuda")[:, None], par)
+    assert torch.equal(reorder_states(x.conj(), par), x.conj().resolve_conj()[at])
+    y = x[:, :, 0].conj().imag  # a lazily negated view
+    assert torch.equal(reorder_states(y, par), y.clone()[at])

@@ -218,16 +218,24 @@ __global__ __launch_bounds__(256) void beam_chunk_kernel(const T* __restrict__ l
     }
 }
 
+// A value, and what decides between equal ones.  Of two words of a beam the one with the larger logit is ahead, also where 64 bits
+// cannot tell score + (logit - lse) apart (fp32 logits of 1e-18, a score of -1e30); else the lower beam, then the lower word.
+// This is the order in which a chunk's list is sorted.
 struct Pick {
     double v;
-    uint32_t at;
+    uint64_t tie;  // beam, the logit's place from above, word
 };
-__device__ __forceinline__ bool ahead(const Pick& a, const Pick& b) { return (a.v > b.v) | ((a.v == b.v) & (a.at < b.at)); }
+constexpr int WORD_BITS = 25;  // SEL_MAX_LISTS chunks of twice SEL_CHUNK words at most
+static_assert((int64_t)SEL_MAX_LISTS * 2 * SEL_CHUNK <= 1 << WORD_BITS && SEL_MAX_BEAMS <= 1 << (64 - 32 - WORD_BITS), "does not fit a tie");
+__device__ __forceinline__ uint64_t tie_of(int k, uint32_t ord, uint32_t word) {
+    return (uint64_t)k << (32 + WORD_BITS) | (uint64_t)(0xffffffffu - ord) << WORD_BITS | word;
+}
+__device__ __forceinline__ bool ahead(const Pick& a, const Pick& b) { return (a.v > b.v) | ((a.v == b.v) & (a.tie < b.tie)); }
 
-// One workgroup per utterance: the row sums in 64 bits, then the best n of the chunks' sorted lists.  Values are
-// compared in 64 bits, where different logits of a beam stay different (and equal ones equal); the n-th best list head
-// bounds the n-th best value from below, so at most n lists of at most n keys are candidates.  Bound by its chain of
-// dependent steps: everything it may need is loaded first (a load is about a microsecond, the arithmetic is less).
+// One workgroup per utterance: the row sums in 64 bits, then the best n of the chunks' sorted lists.  Values are compared in 64
+// bits; the n-th best list head bounds the n-th best value from below, so at most n lists of at most n keys are candidates.
+// Bound by its chain of dependent steps: everything it may need is loaded first (a load is about a microsecond, the arithmetic
+// is less).
 constexpr int JOIN_T = 512;
 constexpr int JOIN_HELD = 4;  // keys per thread that are loaded ahead: all of them up to 2048
 __device__ __forceinline__ int over(int x, float inverse) { return (int)(((float)x + 0.5f) * inverse); }  // exact: x < 2^16, divisors up to 2048
@@ -249,13 +257,13 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
     __shared__ double score[SEL_MAX_BEAMS];
     __shared__ int alive[SEL_MAX_BEAMS];
     __shared__ double head_v[SEL_MAX_LISTS];
-    __shared__ uint32_t head_at[SEL_MAX_LISTS];
+    __shared__ uint64_t head_tie[SEL_MAX_LISTS];
     __shared__ double cand_v[SEL_MAX_N * SEL_MAX_N];
-    __shared__ uint32_t cand_at[SEL_MAX_N * SEL_MAX_N];
+    __shared__ uint64_t cand_tie[SEL_MAX_N * SEL_MAX_N];
     __shared__ Pick tau;
     __shared__ int n_cand;
     __shared__ double best_v[SEL_MAX_N];
-    __shared__ uint32_t best_at[SEL_MAX_N];
+    __shared__ uint64_t best_tie[SEL_MAX_N];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int b = blockIdx.x;
     const int lists = K * chunks, all = lists * n;
@@ -268,7 +276,7 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
     }
     if (threadIdx.x == 0) {
         n_cand = 0;
-        tau = Pick{-__builtin_inf(), 0xffffffffu};  // everything is ahead of it
+        tau = Pick{-__builtin_inf(), ~0ull};  // everything is ahead of it
     }
     for (int k = wave; k < K; k += JOIN_T / 64) {
         const float2* st = stats + ((int64_t)b * K + k) * chunks * SEL_WAVES;
@@ -303,10 +311,10 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
     auto entry = [&](int l, int j, uint64_t key, Pick& p) -> bool {
         const int k = over(l, chunks_inv);
         if (!alive[k]) {  // a dead beam: its words in order
-            p = Pick{-__builtin_inf(), (uint32_t)(k * V + j)};
+            p = Pick{-__builtin_inf(), tie_of(k, 0, j)};
             return l == k * chunks && j < V;
         }
-        p = Pick{score[k] + ((double)unord32((uint32_t)(key >> 32)) - lse[k]), (uint32_t)(k * V) + (0xffffffffu - (uint32_t)key)};
+        p = Pick{score[k] + ((double)unord32((uint32_t)(key >> 32)) - lse[k]), tie_of(k, (uint32_t)(key >> 32), 0xffffffffu - (uint32_t)key)};
         return key != 0;
     };
     auto each = [&](auto&& f) __attribute__((always_inline)) {  // f(list, place in it, key)
@@ -320,16 +328,16 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
         Pick p;
         const bool any = entry(l, 0, key, p);
         head_v[l] = any ? p.v : __builtin_nan("");
-        head_at[l] = any ? p.at : 0xffffffffu;
+        head_tie[l] = any ? p.tie : ~0ull;
     });
     __syncthreads();
     const int part = threadIdx.x & 3;  // four threads per head, and per candidate, each against a quarter of the others
     for (int l = threadIdx.x >> 2; l < lists; l += JOIN_T / 4) {
-        const Pick p{head_v[l], head_at[l]};
+        const Pick p{head_v[l], head_tie[l]};
         int r = 0;
         for (int u0 = part; u0 < lists; u0 += 16)
 #pragma unroll
-            for (int u = u0; u < u0 + 16; u += 4) r += (u < lists) & ahead(Pick{head_v[u], head_at[u]}, p);  // NaN is ahead of nothing
+            for (int u = u0; u < u0 + 16; u += 4) r += (u < lists) & ahead(Pick{head_v[u], head_tie[u]}, p);  // NaN is ahead of nothing
         r += __shfl_xor(r, 1, 64);
         r += __shfl_xor(r, 2, 64);
         if (part == 0 && r == n - 1 && p.v == p.v) tau = p;
@@ -337,33 +345,33 @@ __global__ __launch_bounds__(JOIN_T) void beam_join_kernel(const uint64_t* __res
     __syncthreads();
     const Pick least = tau;
     each([&](int l, int j, uint64_t key) {
-        if (head_v[l] != head_v[l] || ahead(least, Pick{head_v[l], head_at[l]})) return;
+        if (head_v[l] != head_v[l] || ahead(least, Pick{head_v[l], head_tie[l]})) return;
         Pick p;
         if (!entry(l, j, key, p) || ahead(least, p)) return;
         const int at = atomicAdd(&n_cand, 1);
         cand_v[at] = p.v;
-        cand_at[at] = p.at;
+        cand_tie[at] = p.tie;
     });
     __syncthreads();
     const int c = n_cand;
     for (int t = threadIdx.x >> 2; t < c; t += JOIN_T / 4) {
-        const Pick p{cand_v[t], cand_at[t]};
+        const Pick p{cand_v[t], cand_tie[t]};
         int r = 0;
         for (int u0 = part; u0 < c; u0 += 16)
 #pragma unroll
-            for (int u = u0; u < u0 + 16; u += 4) r += (u < c) & ahead(Pick{cand_v[u], cand_at[u]}, p);
+            for (int u = u0; u < u0 + 16; u += 4) r += (u < c) & ahead(Pick{cand_v[u], cand_tie[u]}, p);
         r += __shfl_xor(r, 1, 64);
         r += __shfl_xor(r, 2, 64);
         if (part == 0 && r < n) {
             best_v[r] = p.v;
-            best_at[r] = p.at;
+            best_tie[r] = p.tie;
         }
     }
     __syncthreads();
     if (wave == 0) {  // n <= 32 lanes
         const bool in = lane < n;
-        const uint32_t at = in ? best_at[lane] : 0;
-        const int64_t parent = at / (uint32_t)V, token = at % (uint32_t)V;
+        const uint64_t tie = in ? best_tie[lane] : 0;
+        const int64_t parent = tie >> (32 + WORD_BITS), token = tie & ((1 << WORD_BITS) - 1);
         const float v = in ? (float)best_v[lane] : 0.f;
         if (in) {
             cand_scores[(int64_t)b * n + lane] = v;

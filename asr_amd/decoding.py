@@ -79,8 +79,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, eos_token_id: Option
 
     ``logits`` [B*K, V] or [B, K, V] (float32 or bfloat16; rows may lie at any stride, as those of a padded output layer
     or of the last position of a longer run), ``scores`` float32 [B, K] (-inf: no beam).  A continuation's value is
-    ``scores[b, k] + log_softmax(logits[b, k])[v]``, ordered best first, ties to the lowest ``k * V + v``.  -inf logits
-    are words that cannot follow.  A beam whose score or largest logit is not finite, or that has a NaN logit, offers only
+    ``scores[b, k] + log_softmax(logits[b, k])[v]``, ordered best first, ties to the lowest ``k * V + v`` (values are
+    compared in 64 bits; of two words of one beam the larger logit is ahead even where 64 bits cannot tell them apart).  -inf
+    logits are words that cannot follow.  A beam whose score or largest logit is not finite, or that has a NaN logit, offers only
     -inf.  Continuations with ``eos_token_id`` are among the 2K candidates but do not go on.  1 <= K <= 16, V >= 2."""
     if scores.dim() != 2 or scores.dtype != torch.float32:
         raise ValueError("scores must be a float32 [B, K] tensor")

@@ -247,10 +247,11 @@ int asrk_attention_log2_bf16(const void* qkv, void* out, int B, int T, int H, vo
  * ---------------------------------------------------------------------------------------- */
 
 /* The best 2 K of the K V continuations of each utterance, c = scores[b][k] + log_softmax(logits[b K + k])[v], best
- * first and ties to the lowest k V + v, as cand_* [B][2 K]; and the first K of them whose token is not `eos` (< 0: none),
- * as out_* [B][K].  logits dev [B K] rows of V values (ASRK_F32 | ASRK_BF16) at a stride of ld values; scores dev f32
- * [B][K].  Beams whose score or largest logit is not finite, or with a NaN logit, offer -inf.  K <= 16, 2 <= V,
- * K V < 2^31, K ceil(V / 8192) <= 2048.  ws: dev scratch, 16-byte aligned. */
+ * first and ties to the lowest k V + v (compared in 64 bits; the words of one beam by their logits also where 64 bits cannot
+ * tell their c apart), as cand_* [B][2 K]; and the first K of them whose token is not `eos` (< 0: none), as out_* [B][K].
+ * logits dev [B K] rows of V values (ASRK_F32 | ASRK_BF16) at a stride of ld values; scores dev f32 [B][K].  Beams whose score
+ * or largest logit is not finite, or with a NaN logit, offer -inf.  K <= 16, 2 <= V, K V < 2^31, K ceil(V / 8192) <= 2048.
+ * ws: dev scratch, 16-byte aligned. */
 size_t asrk_beam_select_workspace_bytes(int B, int K, int V);
 int asrk_beam_select(const void* logits, int dtype, int64_t ld, const float* scores, int B, int K, int V, int64_t eos,
                      float* out_scores, int64_t* out_tokens, int64_t* out_parents, float* cand_scores, int64_t* cand_tokens,

@@ -11,19 +11,22 @@ EXP_MIN, EXP_MAX = -64, 119
 
 
 def select(logits, scores, eos=-1):
-    """logits [B, K, V], scores [B, K] -> (scores, tokens, parents) of the K that go on, and of the best 2K."""
+    """logits [B, K, V], scores [B, K] -> (scores, tokens, parents) of the K that go on, and of the best 2K.  Values that are equal
+    in 64 bits: the lowest beam first, within a beam the largest logit (values that differ by less than 64 bits tell are equal,
+    their logits are not), then the lowest word."""
     x = np.asarray(logits, np.float64)
     s = np.asarray(scores, np.float64)
     B, K, V = x.shape
     out = [np.zeros((B, n), t) for n in (K, 2 * K) for t in (np.float64, np.int64, np.int64)]
     for b in range(B):
-        value = np.full((K, V), -np.inf)
+        value, logit = np.full((K, V), -np.inf), np.zeros((K, V))
         for k in range(K):
             top = x[b, k].max()
             if np.isfinite(top) and np.isfinite(s[b, k]) and not np.isnan(x[b, k]).any():
                 value[k] = s[b, k] + (x[b, k] - (top + math.log(np.exp(x[b, k] - top).sum())))
+                logit[k] = x[b, k]
         flat = value.reshape(-1)
-        order = np.argsort(-flat, kind="stable")[:2 * K]
+        order = np.lexsort((-logit.reshape(-1), np.repeat(np.arange(K), V), -flat))[:2 * K]  # stable: then by word
         go = [i for i in order if i % V != eos][:K]
         for j, picks in ((0, go), (3, order)):
             out[j][b], out[j + 1][b], out[j + 2][b] = flat[picks], [i % V for i in picks], [i // V for i in picks]

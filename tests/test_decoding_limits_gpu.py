@@ -179,6 +179,34 @@ def test_write_takes_any_stride_of_a_dimension_of_one():
 # ---- selection
 
 
+@pytest.mark.parametrize("V", [41, 1000, 9001, 20001])
+@pytest.mark.parametrize("what", ["tiny logits", "enormous scores", "one of them tiny"])
+def test_select_orders_words_that_64_bits_cannot_tell_apart(V, what):
+    """score + (logit - lse) is the same number for many words: within a beam their logits decide."""
+    from asr_amd.decoding import beam_select
+
+    g = _gen(V)
+    B, K = 3, 4
+    x = torch.randn((B * K, V), generator=g, device="cuda")
+    s = -torch.rand((B, K), generator=g, device="cuda") * 3
+    if what == "tiny logits":
+        x *= 1e-18
+    elif what == "enormous scores":
+        s -= 2.0 ** 100
+    else:
+        x[::2] *= 1e-18
+        x[1::2] = x[1::2].clamp(max=0.25)
+    s[0, 1] = s[0, 0]
+    s[2, 3] = -math.inf
+    for eos in (None, 0):
+        got = [t.cpu().numpy() for t in beam_select(x, s, eos)]
+        want = od.select(x.view(B, K, V).double().cpu().numpy(), s.double().cpu().numpy(), -1 if eos is None else eos)
+        for i in (1, 2, 4, 5):
+            assert np.array_equal(got[i], want[i]), (i, got[i], want[i])
+        for i in (0, 3):
+            assert np.allclose(got[i], want[i], rtol=2.0 ** -24, atol=1e-5)
+
+
 def test_reorder_states_of_conjugated_and_negated_views():
     from asr_amd.decoding import reorder_states
 

@@ -150,10 +150,11 @@ def reorder_states(states: torch.Tensor, parents: torch.Tensor) -> torch.Tensor:
 class PagedKVCache:
     """Keys and values of ``num_seqs`` sequences in 8 bits, on pages of 64 tokens.
 
-    A page of one key/value head holds e4m3 values with one power-of-two scale for its keys and one for its values: the
-    smallest that fits its tokens, so that a value is off by at most 2**-4 of itself (or 2**-10 of ``2**e``, where it is
-    that small).  When a later token of the page needs a larger scale, the older ones are rounded to it again.  NaN and
-    infinities are kept as NaN.
+    A page of one key/value head holds e4m3 values with one power-of-two scale ``2**e`` for its keys and one for its values: the
+    smallest that fits its tokens.  A value is off by at most 2**-4 of itself, or where it is that small by 2**-10 of ``2**e``.
+    When a later token of the page needs a larger scale, the older ones are rounded to it again: exactly, but for the small
+    ones, whose roundings add up to less than 2**-9 of ``2**e``.  ``e`` lies in -64 .. 119: magnitudes above 1.75 * 2**127
+    become that.  NaN and infinities are kept as NaN.
 
         cache = PagedKVCache(B * K, max_len, kv_heads, head_dim, num_layers=L, device="cuda")
         prompts = cache.leaders(K)                # every K-th sequence: one per utterance
@@ -343,6 +344,8 @@ class PagedKVCache:
         shape (any strides; query head j reads key/value head ``j // (q_heads // kv_heads)``).  Row i of sequence s sees the
         tokens up to its own, ``starts[s] + i``; rows behind ``lens[s]`` are zero.  Tokens that a row sees have to have been written;
         those behind the last row's own need not be yet.  ``scale`` (positive) is ``head_dim ** -0.5`` by default.
+
+        The weights of the tokens are held to 2**-11 of themselves, and below 2**-27 of a row's largest to 2**-38 of that.
 
         ``num_beams`` consecutive sequences are worked on together, and pages that they share are read once.  It changes
         no result but for rounding: the beams may share any pages, or none."""

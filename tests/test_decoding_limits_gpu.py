@@ -176,6 +176,30 @@ def test_write_takes_any_stride_of_a_dimension_of_one():
                 same_tokens(c, o, 0, 70)
 
 
+def test_held_values_are_as_near_as_documented():
+    """A value is off by at most 2**-4 of itself, or by less than 2**-9 of 2**e where it is that small, however often its page's
+    scale has grown (and may be off by more than 2**-10 of 2**e then)."""
+    from asr_amd.decoding import PagedKVCache
+
+    c = PagedKVCache(1, 64, 1, 64)
+    x = torch.zeros((1, 64, 1, 64), device="cuda")
+    x[0, 0, 0] = torch.linspace(0.0, 8.0, 64, device="cuda") * 2.0 ** -9
+    x[0, 0, 0, 0], x[0, 0, 0, 1] = 448.0, 2.51 * 2.0 ** -9  # e = 0, then a tie at e = 1
+    worst = 0.0
+    for t in range(10):
+        if t:
+            x[0, t] = torch.rand((1, 64), generator=_gen(t), device="cuda") * 2.0 ** (t - 9)
+            x[0, t, 0, 0] = 448.0 * 2.0 ** t
+        c.extend(1)
+        c.write(x[:, t:t + 1], x[:, t:t + 1])
+        for held in c.read(0, t + 1, layer=0):
+            off = (held.double() - x[:, :t + 1].double()).abs()
+            assert bool(((off <= x[:, :t + 1].double() * 2.0 ** -4) | (off < 2.0 ** (t - 9))).all()), t
+            small = off[x[:, :t + 1] < 2.0 ** (t - 6)]
+            worst = max(worst, float(small.max()) / 2.0 ** (t - 10))
+    assert 1.0 < worst < 2.0
+
+
 # ---- selection
 
 

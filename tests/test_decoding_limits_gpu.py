@@ -153,6 +153,56 @@ def test_attend_before_the_last_new_tokens_are_written(beams, before, rows, n, g
     same_attention(c, o, q, beams=beams)
 
 
+def test_as_many_sequences_as_a_cache_takes():
+    """65535 sequences: every step of a search."""
+    from asr_amd.decoding import PagedKVCache
+
+    S, K = 65535, 5
+    c = PagedKVCache(S, 64, 1, 64)
+    g = _gen(65535)
+    n = torch.randint(0, 4, (S,), generator=g, device="cuda")
+    k, v = (torch.randn((S, 3, 1, 64), generator=g, device="cuda").bfloat16() for _ in range(2))
+    c.extend(n)
+    c.write(k, v)
+    c.check()
+    assert torch.equal(c.lens.long(), n) and int((c.refs > 0).sum()) == int((n > 0).sum()) == int(c.table.max()) + 1
+    held = c.read(0, 4, layer=0)
+    par = torch.randint(0, K, (S // K, K), generator=g, device="cuda")
+    c.reorder(par)
+    src = (torch.arange(S // K, device="cuda")[:, None] * K + par).view(-1)
+    for got, want in zip(c.read(0, 4, layer=0), held):
+        assert torch.equal(got, want[src])
+    c.extend(1)
+    k1, v1 = (torch.randn((S, 1, 1, 64), generator=g, device="cuda").bfloat16() for _ in range(2))
+    c.write(k1, v1)
+    c.check()
+    q = torch.randn((S, 1, 2, 64), generator=g, device="cuda").bfloat16()
+    got = c.attend(q, num_beams=K)
+    assert int(c.compact()) == int((c.refs > 0).sum())
+    assert torch.equal(c.attend(q, num_beams=K), got) and torch.equal(c.attend(q), got)
+    keys, values = (x.double() for x in c.read(0, 4, layer=0))
+    seen = torch.arange(4, device="cuda") < c.lens[:, None]
+    p = ((q[:, 0].double()[:, :, None] * keys[:, None, :, 0]).sum(3) / 8).masked_fill(~seen[:, None], -math.inf).softmax(2)
+    want, size = ((p[..., None] * x[:, None, :, 0]).sum(2) for x in (values, values.abs()))
+    assert bool(((got[:, 0].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * size).all())
+
+
+def test_as_many_rows_as_one_call_takes():
+    """65535 workgroups of 128 rows over one sequence: the rows behind its last token are zero, also the very last."""
+    rng = np.random.default_rng(1)
+    c, o = both(1, 300, 1, 64)
+    for rows in (100, 150):
+        c.extend(rows)
+        o.extend(rows)
+        put(c, o, normal(rng, 1, rows, 1, 64), normal(rng, 1, rows, 1, 64))
+    q = torch.from_numpy(rng.standard_normal((1, 150, 1, 64))).cuda().bfloat16()
+    same_attention(c, o, q)
+    many = torch.zeros((1, 65535 * 128, 1, 64), device="cuda", dtype=torch.bfloat16)
+    many[:, :150] = q
+    got = c.attend(many)
+    assert torch.equal(got[:, :150], c.attend(q)) and int((got[:, 150:] != 0).sum()) == 0
+
+
 # ---- tokens
 
 
@@ -240,3 +290,17 @@ def test_reorder_states_of_conjugated_and_negated_views():
     assert torch.equal(reorder_states(x.conj(), par), x.conj().resolve_conj()[at])
     y = x[:, :, 0].conj().imag  # a lazily negated view
     assert torch.equal(reorder_states(y, par), y.clone()[at])
+
+
+def test_refusals_of_tensors_on_two_devices():
+    from asr_amd import _lib
+    from asr_amd.decoding import PagedKVCache, beam_select, reorder_states
+
+    x, par = torch.zeros((2, 2, 64), device="cuda"), torch.zeros((2, 2), dtype=torch.int64, device="cuda")
+    c = PagedKVCache(4, 64, 1, 64)
+    rows = torch.zeros((4, 1, 1, 64), device="cuda")
+    for call in (lambda: reorder_states(x.cpu(), par), lambda: reorder_states(x, par.cpu()), lambda: beam_select(x, x[:, :, 0].contiguous().cpu()),
+                 lambda: beam_select(x.cpu(), x[:, :, 0].contiguous()), lambda: c.write(rows, rows.cpu()), lambda: c.write(rows.cpu(), rows)):
+        with pytest.raises(_lib.AsrkError):
+            call()
+    assert int(c.status[0]) == 0

@@ -15,7 +15,7 @@
 // Unit).  Weights are rounded to f16, 2^-11 relative, 8 times finer than bf16 would be and well under the 2^-8 of the bf16
 // result.  Everything else is fp32.
 // Measured: 1.2 GB of cache (48 sequences, 8 heads of 128) 203 us = 5.9 TB/s; 64 x 5 beams over 1641 tokens that share their
-// prompts (64 MB) 19 us; one utterance 11 us, latency, of which fetching the code for the first time is a good part.
+// prompts (64 MB) 20 us; one utterance 11 us, latency, of which fetching the code for the first time is a good part.
 #include "asrk_kvcache.h"
 
 namespace {
@@ -363,7 +363,8 @@ __device__ __forceinline__ void walk_apart(Item item, Pages& work, int pages, co
 }
 
 // The same from the first page on, with nothing of what the other loop holds: if it went on from there, that loop would be cut
-// for both (two spilled registers more in kv_prompt_kernel<64>, 10 % of the time of 16 prompts).  Its presence still costs 1 to 4 %.
+// for both (two spilled registers more in kv_prompt_kernel<64>, 10 % of the time of 16 prompts).  Its presence still costs 1 to 4 %; a call
+// that goes through it takes twice its time.
 template <int D, int CT>
 __device__ __forceinline__ void walk_apart_anew(const asrk_kv_cache& c, const Columns& cs, int first_col, int first_page, int step, int pages,
                                                 const char* layer, const int* exps, float* m, f32x4* l, f32x4 (*o)[D / 16]) {
@@ -575,8 +576,8 @@ void kv_attention_kernel(asrk_kv_cache c, AttnArgs a) {
 // it is vector instructions, and a fifth of those are conversions, so every page is converted once for the four waves: each
 // converts a quarter, into LDS, in the order in which the products' first operands are read (a lane's 16 bytes after
 // another's: no bank conflict).  Two buffers, one barrier per page; the next page's bytes are on their way meanwhile.
-// 16 prompts of up to 1541 tokens, 15 query heads on 5 of 64: 89 us (460 TFLOP/s; every wave converting for itself 105); of 4096
-// tokens 740 TFLOP/s, with heads of 128 835.  Of a wave's vector issue slots 60 % are used: the rest is the prologue of short
+// 16 prompts of up to 1541 tokens, 15 query heads on 5 of 64: 91 us (450 TFLOP/s; every wave converting for itself 105); of 4096
+// tokens 735 TFLOP/s, with heads of 128 780.  Of a wave's vector issue slots 60 % are used: the rest is the prologue of short
 // rows and waves of a workgroup waiting for each other.
 constexpr int PROMPT_W = 4, PROMPT_CT = 2;
 // (D 64: 4 waves per SIMD, a few spilled registers included, are 7 % faster than 3.)
